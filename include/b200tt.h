@@ -445,6 +445,68 @@ int32_t b200_decode_layers(b200_engine*, const b200_decode_shape* shape, b200_bu
                            b200_buffer final_norm, b200_buffer cos_table, b200_buffer sin_table, b200_buffer position,
                            b200_buffer* out, uint64_t out_dims[2]);
 
+/* --- a key/value cache in pages (an extension beside the trait, as `b200_attention_blocks` is).  The reference's cache is
+ * one fixed block of positions a sequence (crates/tt-models/src/kv_cache.rs:5-11); here a layer's cache is a pool of pages of
+ * `page_size` positions, and a table names each sequence's pages, so that sequences of any lengths share the pool:
+ *   key_pages, value_pages  [pages * page_size, kv_heads * head_dim], both F32 or both BF16, position-major in a page as the
+ *                           reference's cache is (one page of max_len positions a sequence IS that cache)
+ *   page_table              I32 [sequences, pages a sequence]: position p of sequence s is row
+ *                           page_table[s, p / page_size] * page_size + p % page_size.  Only entries a call needs are read;
+ *                           the others may hold anything.
+ *   positions               I32, one value a row of the call; -1 marks a padding row or an idle slot.
+ * A position behind the table's last page (or, with a rotation, outside the cos and sin tables) or below -1, a sequence outside
+ * the table or a page number outside the pool sets DOMAIN on the device: the row is then treated as padding (in attention, a
+ * page outside the pool is left out and the others attended), and nothing outside the buffers is touched.  `into` is 0 or a live buffer of the result's dims and element type at a
+ * 16-byte address that shares no memory with the call's other buffers: the result is then written there (and *out = into)
+ * instead of into a new buffer. */
+typedef struct { uint32_t heads, kv_heads, head_dim, page_size; } b200_page_shape;
+/* The rotation of `rope_blocks` (server.rs:566) on a projection's query and key heads and the cache write of
+ * `scatter_rows_into` (server.rs:389) as one pass: qkv is a block [n, (heads + 2 kv_heads) head_dim] (Wq | Wk | Wv side by
+ * side, F32 or BF16); its row i is the token at positions[i] of sequence sequences[i] (0 in place of `sequences`: of sequence
+ * i).  cos_table and sin_table are F32 [positions, r] (sin as [-sin, sin]), r even and at most head_dim: columns below r of a
+ * head become fl(fl(x cos) + fl(swap(x) sin)), the others stay; 0 for both: no rotation.  The rotated keys and the values are
+ * rounded once to the cache's type.  The result [n, heads * head_dim] holds the rotated query heads and, with keys_out, the
+ * rotated key heads behind them ([n, (heads + kv_heads) head_dim]: what `rope_blocks` of those columns gives), F32 or BF16.
+ * A padding row writes nothing into the cache, and its row of the result is zero.  No two rows of a call may name the same
+ * position of the same sequence (which of the two would stay is not defined).  Refused unless heads is a multiple of
+ * kv_heads and the pages are whole. */
+int32_t b200_rope_append_pages(b200_engine*, const b200_page_shape* shape, const b200_block_arg* qkv, b200_buffer cos_table,
+                               b200_buffer sin_table, b200_buffer positions, b200_buffer sequences, b200_buffer page_table,
+                               b200_buffer key_pages, b200_buffer value_pages, int32_t keys_out, int32_t out_bf16,
+                               b200_buffer into, b200_buffer* out, uint64_t out_dims[2]);
+/* Attention of one new token a sequence over its pages: `attention_rows` (server.rs:257) with a length a sequence.  q is a
+ * block [n, heads * head_dim] (F32 or BF16), row i the token at positions[i] of sequence i, whose own key and value are in
+ * the cache already; query head h reads key/value head h / (heads / kv_heads).  It attends to positions 0 .. positions[i], or
+ * with window > 0 to the last `window` of them.  out [n, heads * head_dim] = softmax(scale q K^T) V with `attention_rows`'
+ * steps in F32 (clamped maximum and sum: a row that attends to nothing, positions[i] == -1 or scores all -inf, is zero),
+ * rounded once with out_bf16.  Nothing behind a sequence's last position is read.  Refused unless head_dim is 32, 64, 96,
+ * 128, 192 or 256 and heads is a multiple of kv_heads. */
+int32_t b200_attention_pages(b200_engine*, const b200_page_shape* shape, const b200_block_arg* q, b200_buffer key_pages,
+                             b200_buffer value_pages, b200_buffer page_table, b200_buffer positions, uint32_t window, float scale,
+                             int32_t out_bf16, b200_buffer into, b200_buffer* out, uint64_t out_dims[2]);
+
+/* --- log probabilities of given tokens (an extension beside the trait: burn-tt composes log_softmax and gather,
+ * ops.rs:5153-5158 and :1001).  logits [rows, vocab] F32 or BF16, y = scale * logits, ids I32 of rows values:
+ *   out[0] F32 [rows, 1]  y[id] - lse (0 where id is -1: a padding row or a row without a given token)
+ *   out[1] F32 [rows, 1]  the entropy -sum p log p of p = softmax(y); an entry of -inf adds nothing
+ *   out[2] F32 [rows, 1]  lse = log sum exp(y)
+ *   out[3] I32 [rows, top], out[4] F32 [rows, top] (with top > 0; else 0): the `top` largest logits' columns, largest first and
+ *                         equal values by the lower column, NaN above everything (`argmax_row`'s order), and their y - lse
+ * One pass over the logits; sums in F32 under the row's maximum.  A row of -inf only has lse -inf, entropy 0 and log
+ * probabilities -inf; a row with a NaN or +inf has NaN in all three.  Another id outside the columns sets DOMAIN (and gives 0).
+ * `into` is NULL or five ids as `b200_rope_append_pages` takes one (0: a new buffer).  Refused unless scale is positive and
+ * finite, top <= 32 and top <= vocab. */
+int32_t b200_token_logprobs(b200_engine*, b200_buffer logits, b200_buffer ids, float scale, uint32_t top, const b200_buffer into[5],
+                            b200_buffer out[5], uint64_t out_dims[2]);
+/* The gradient of the first two with respect to the logits: with p = exp(y - lse) and the rows' upstream gradients
+ * d_logprob and d_entropy (F32, rows values; d_entropy and entropy 0: absent),
+ *   out = scale * (d_logprob (1[column = id] - p) - d_entropy p (y - lse + entropy)),
+ * F32 or rounded once to BF16, [rows, vocab].  lse and entropy are the forward's.  A row whose id is -1 has no d_logprob
+ * term; an entry of -inf has gradient 0 (its own 1[column = id] term apart), a row of -inf only is zero. */
+int32_t b200_token_logprobs_backward(b200_engine*, b200_buffer logits, b200_buffer ids, b200_buffer lse, b200_buffer entropy,
+                                     b200_buffer d_logprob, b200_buffer d_entropy, float scale, int32_t out_bf16,
+                                     b200_buffer into, b200_buffer* out, uint64_t out_dims[2]);
+
 /* --- traces: server.rs:591 `begin_trace`, :595 `end_trace`, :650 `run_trace`, :660 `release_trace`.
  * Ops issued between begin and end are captured into a CUDA graph instead of running; a replay
  * runs them again on the same buffers.  Inputs are buffers made before the capture (refresh them

@@ -27,6 +27,7 @@ COMMON = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "-Xcompiler",
 # source -> extra flags.  -fmad=false where the reference defines separate roundings.
 SOURCES = {
     "engine.cu": ["-Xcompiler", "-fvisibility=default"],
+    "engine_serving.cu": ["-Xcompiler", "-fvisibility=default"],
     "k_eltwise.cu": ["-fmad=false"],
     "k_reduce.cu": ["-fmad=false"],
     "k_index.cu": [],
@@ -41,6 +42,8 @@ SOURCES = {
     "k_convert.cu": [],
     "k_bfp.cu": [],
     "k_decode.cu": [],
+    "k_pages.cu": [],
+    "k_logprob.cu": [],
     "k_pool.cu": ["-fmad=false"],
     "k_scan_sort.cu": ["-fmad=false"],
     "k_random.cu": ["-fmad=false"],

@@ -244,4 +244,69 @@ cudaError_t ensure_dynamic_smem(const void* kernel, size_t bytes);
 bool device_value_get(const void* key, int* value);
 void device_value_set(const void* key, int value);
 
+// ---- the paged cache (k_pages.cu) -----------------------------------------------
+// The cache of one layer as a kernel sees it: position p of sequence s is row table[s, p / page] * page + p % page.
+struct PageView {
+  const int32_t* table = nullptr;
+  uint32_t sequences = 0, width = 0;       // the table's rows and columns
+  void *keys = nullptr, *values = nullptr;
+  int bf16 = 0;
+  uint32_t pages = 0, page = 0;            // pages in the pool, positions a page
+  uint32_t heads = 0, kv_heads = 0, dim = 0;
+};
+struct AppendArgs {
+  PageView cache;
+  Mat qkv;                                 // [n, (heads + 2 kv_heads) dim]
+  const float *cos = nullptr, *sin = nullptr;   // [table_rows, rotary]
+  uint64_t table_rows = 0;
+  uint32_t rotary = 0;
+  const int32_t *positions = nullptr, *sequences = nullptr;   // sequences null: row i is sequence i
+  uint64_t n = 0;
+  int keys_out = 0;
+  void* out = nullptr;
+  int out_bf16 = 0;
+  int* err = nullptr;
+};
+cudaError_t launch_rope_append_pages(const AppendArgs& args, cudaStream_t stream);
+struct AttnPagesArgs {
+  PageView cache;
+  Mat q;                                   // [n, heads dim]
+  const int32_t* positions = nullptr;
+  uint64_t n = 0;
+  uint32_t window = 0;
+  float scale = 1.f;
+  void* out = nullptr;
+  int out_bf16 = 0;
+  int* err = nullptr;
+};
+bool attention_pages_dim_ok(uint32_t dim);
+cudaError_t launch_attention_pages(const AttnPagesArgs& args, cudaStream_t stream);
+
+// ---- token log probabilities (k_logprob.cu) -------------------------------------
+struct LogprobArgs {
+  const void* logits = nullptr;
+  int bf16 = 0;
+  uint64_t rows = 0, cols = 0;
+  const int32_t* ids = nullptr;
+  float scale = 1.f;
+  uint32_t top = 0;
+  float *logprob = nullptr, *entropy = nullptr, *lse = nullptr;
+  int32_t* top_ids = nullptr;
+  float* top_logprobs = nullptr;
+  int* err = nullptr;
+};
+cudaError_t launch_token_logprobs(const LogprobArgs& args, cudaStream_t stream);
+struct LogprobGradArgs {
+  const void* logits = nullptr;
+  int bf16 = 0;
+  uint64_t rows = 0, cols = 0;
+  const int32_t* ids = nullptr;
+  const float *lse = nullptr, *entropy = nullptr, *d_logprob = nullptr, *d_entropy = nullptr;   // entropy, d_entropy: null when absent
+  float scale = 1.f;
+  void* out = nullptr;
+  int out_bf16 = 0;
+  int* err = nullptr;
+};
+cudaError_t launch_token_logprobs_backward(const LogprobGradArgs& args, cudaStream_t stream);
+
 }  // namespace b200

@@ -86,6 +86,10 @@ class DecodeShape(C.Structure):  # b200_decode_shape
                [("eps", C.c_float), ("scale", C.c_float)]
 
 
+class PageShape(C.Structure):  # b200_page_shape
+    _fields_ = [(n, C.c_uint32) for n in ("heads", "kv_heads", "head_dim", "page_size")]
+
+
 class OpStat(C.Structure):  # burn-tt/src/report.rs:27 `OpStat`, reduced (b200_op_stat)
     _fields_ = [("op", C.c_char * 48), ("calls", C.c_uint64), ("launches", C.c_uint64), ("device_ms", C.c_double)]
 
@@ -699,6 +703,45 @@ class CudaEngine:
         return self._call(self._lib.b200_decode_layers, C.byref(shape), C.c_uint64(x), ids, C.c_uint64(final_norm), C.c_uint64(cos),
                           C.c_uint64(sin), C.c_uint64(position))
 
+    # -- the paged cache and token log probabilities (extensions beside the trait) -------------
+    def rope_append_pages(self, shape: "PageShape", qkv, cos: Optional[int], sin: Optional[int], positions: int, sequences: Optional[int],
+                          page_table: int, key_pages: int, value_pages: int, keys: bool = False, bf16: bool = False, into: int = 0) -> Out:
+        """RoPE on a projection's query and key heads and the cache write as one pass (`b200_rope_append_pages`): qkv is a
+        block [n, (heads + 2 kv_heads) head_dim]; row i is the token at positions[i] of sequence sequences[i] (None: of
+        sequence i), -1 a padding row.  Returns the rotated query heads, with `keys` the rotated key heads behind them."""
+        b = _block(qkv)
+        return self._call(self._lib.b200_rope_append_pages, C.byref(shape), C.byref(b), C.c_uint64(cos or 0), C.c_uint64(sin or 0),
+                          C.c_uint64(positions), C.c_uint64(sequences or 0), C.c_uint64(page_table), C.c_uint64(key_pages),
+                          C.c_uint64(value_pages), C.c_int32(1 if keys else 0), C.c_int32(1 if bf16 else 0), C.c_uint64(into))
+
+    def attention_pages(self, shape: "PageShape", q, key_pages: int, value_pages: int, page_table: int, positions: int, scale: float,
+                        window: int = 0, bf16: bool = False, into: int = 0) -> Out:
+        """One new token's attention over its sequence's pages (`b200_attention_pages`): q is a block
+        [n, heads head_dim], row i the token at positions[i] of sequence i (-1: an idle slot, a row of zeros); `window` > 0
+        keeps the last `window` positions.  Returns [n, heads head_dim]."""
+        b = _block(q)
+        return self._call(self._lib.b200_attention_pages, C.byref(shape), C.byref(b), C.c_uint64(key_pages), C.c_uint64(value_pages),
+                          C.c_uint64(page_table), C.c_uint64(positions), C.c_uint32(window), C.c_float(scale), C.c_int32(1 if bf16 else 0),
+                          C.c_uint64(into))
+
+    def token_logprobs(self, logits: int, ids: int, scale: float = 1.0, top: int = 0, into: Optional[Sequence[int]] = None):
+        """(logprob, entropy, lse) [rows, 1] of the given tokens under softmax(scale * logits), and with `top` > 0 the
+        (columns, log probabilities) [rows, top] of the largest logits (`b200_token_logprobs`): three or five (id, dims)."""
+        out = (C.c_uint64 * 5)()
+        dims = (C.c_uint64 * 2)()
+        dst = None
+        if into is not None:
+            dst = (C.c_uint64 * 5)(*into)
+        self._check(self._lib.b200_token_logprobs(self._e, C.c_uint64(logits), C.c_uint64(ids), C.c_float(scale), C.c_uint32(top), dst, out, dims))
+        rows = dims[0]
+        return [(out[i], (rows, 1 if i < 3 else top)) for i in range(5 if top else 3)]
+
+    def token_logprobs_backward(self, logits: int, ids: int, lse: int, entropy: Optional[int], d_logprob: int, d_entropy: Optional[int] = None,
+                                scale: float = 1.0, bf16: bool = False, into: int = 0) -> Out:
+        """The gradient of `token_logprobs`' log probabilities (and, with d_entropy, entropies) with respect to the logits."""
+        return self._call(self._lib.b200_token_logprobs_backward, C.c_uint64(logits), C.c_uint64(ids), C.c_uint64(lse), C.c_uint64(entropy or 0),
+                          C.c_uint64(d_logprob), C.c_uint64(d_entropy or 0), C.c_float(scale), C.c_int32(1 if bf16 else 0), C.c_uint64(into))
+
     def set_matmul_sm_limit(self, sms: int):
         """Tensor-core products use at most `sms` SMs (0 = all): room for a collective beside them."""
         self._lib.b200_set_matmul_sm_limit(self._e, C.c_int32(sms))
@@ -813,7 +856,7 @@ class CudaEngine:
         return self._lib.b200_stream(self._e)
 
 
-__all__ = ["CudaEngine", "TtError", "EltwiseOp", "Block", "BlockMove", "BlockArg", "BatchedLayout", "Traffic", "OpStat",
+__all__ = ["CudaEngine", "TtError", "EltwiseOp", "Block", "BlockMove", "BlockArg", "BatchedLayout", "Traffic", "OpStat", "PageShape",
            "load_library", "library_path", "kinds",
            "F32", "I32", "BOOL", "BF16", "BFP8", "SUM", "MAX", "PROD", "ALL", "ANY", "BITOR", "SUM_I32", "PROD_I32",
            "MIN_I32", "MAX_I32", "ROWS", "COLS"]
