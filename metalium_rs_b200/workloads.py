@@ -35,10 +35,13 @@ class MlpStep:
     """x [n,784] -> Linear(784,h) -> ReLU -> Linear(h,10) -> softmax cross-entropy, backward, SGD.
     Weights live on the device and are replaced by their updates each step."""
 
-    def __init__(self, eng, w1, b1, w2, b2, lr=0.01, fused_add_relu=True, in_place=False):
+    def __init__(self, eng, w1, b1, w2, b2, lr=0.01, fused_add_relu=True, in_place=False, fused_loss=False):
+        # fused_loss: the loss's log probabilities and their gradient as one op each (`token_logprobs`), where the
+        # composition takes eleven launches and five [n, classes] tensors between them
         # in_place: the update is copied over the old weights, so they keep their addresses
         # (what a captured trace needs to train when it is replayed)
         self.eng, self.lr, self.fused, self.in_place = eng, float(lr), fused_add_relu, in_place
+        self.fused_loss = fused_loss
         self.trace = None
         self.w1 = eng.upload(w1, *w1.shape)
         self.b1 = eng.upload(b1.reshape(1, -1), 1, b1.size)
@@ -61,19 +64,27 @@ class MlpStep:
             t = self._el(K.ADD, pre, self.b1); h = self._el(K.RELU, t); free.append(t)
         z0, _ = e.matmul_dram(h, False, self.w2, False)
         z = self._el(K.ADD, z0, self.b2)
-        logp, _ = e.log_softmax_rows(z)                                            # ops.rs:5153-5158
-        picked, _ = e.pick_columns(logp, labels_buf)                               # ops.rs:1001
+        if self.fused_loss:
+            (picked, _), (ent, _), (lse, _) = e.token_logprobs(z, labels_buf)
+        else:
+            logp, _ = e.log_softmax_rows(z)                                        # ops.rs:5153-5158
+            picked, _ = e.pick_columns(logp, labels_buf)                           # ops.rs:1001
         neg = self._el(K.NEG, picked)
         loss, _ = e.full_sum(neg, mean=True)                                       # ops.rs:3255
         # backward
         zeros, _ = e.zeros_dram((n, 1))
         gval = self._el(K.ADD_SCALAR, zeros, s=-1.0 / n)                           # d(mean(-picked))
-        zl, dims = e.zeros_dram(e.dims_of(logp)[0])
-        g, _ = e.scatter_add_columns(zl, labels_buf, gval)                         # ops.rs:1043
-        p = self._el(K.EXP, logp)                                                  # log-softmax backward:
-        gs, _ = e.reduce(g, SUM, COLS)                                             #   g - exp(logp) * sum(g)
-        pg = self._el(K.MUL, p, gs)
-        dz = self._el(K.SUB, g, pg)
+        if self.fused_loss:
+            dz, _ = e.token_logprobs_backward(z, labels_buf, lse, None, gval)
+            free += [ent, lse]
+        else:
+            zl, dims = e.zeros_dram(e.dims_of(logp)[0])
+            g, _ = e.scatter_add_columns(zl, labels_buf, gval)                     # ops.rs:1043
+            p = self._el(K.EXP, logp)                                              # log-softmax backward:
+            gs, _ = e.reduce(g, SUM, COLS)                                         #   g - exp(logp) * sum(g)
+            pg = self._el(K.MUL, p, gs)
+            dz = self._el(K.SUB, g, pg)
+            free += [logp, zl, g, p, gs, pg]
         dw2, _ = e.matmul_dram(h, True, dz, False)                                 # x^T g (ops.rs:5006-5016)
         db2, _ = e.sum_rows(dz)                                                    # in-order (ops.rs:5022-5028)
         dh, _ = e.matmul_dram(dz, False, self.w2, True)
@@ -89,7 +100,7 @@ class MlpStep:
                 e.copy_into(new, getattr(self, name)); e.free(new)
             else:
                 e.free(getattr(self, name)); setattr(self, name, new)
-        free += [pre, z0, logp, picked, neg, zeros, gval, zl, g, p, gs, pg, dh, h]
+        free += [pre, z0, picked, neg, zeros, gval, dh, h]
         out = {"loss": loss}
         if keep:
             out.update(logits=z, dw1=dw1, db1=db1, dw2=dw2, db2=db2, dz=dz, dpre=dpre)
@@ -233,7 +244,7 @@ class LlamaPrefill:
         self.fused_items = eng.attention_block_array(fused_items)
         self.last_rows = [(0, b * t + t - 1) for b in range(batch)]
 
-    def forward(self, ids_buf: int, all_positions: bool = False, cache: "LlamaDecode" = None, start: int = 0):
+    def forward(self, ids_buf: int, all_positions: bool = False, cache: "LlamaDecode" = None, start: int = 0, lengths=None, slots=None):
         """ids [1, batch*seq] I32 resident.  Returns (logits buffer [batch or batch*seq, vocab] F32,
         argmax buffer I32); the caller frees both.  With `cache`, every layer's rotated keys and its values are
         also written into that generation's cache at positions 0 .. seq-1 of each sequence, as the reference's
@@ -243,14 +254,34 @@ class LlamaPrefill:
         positions start .. start + seq - 1, their keys and values go to those rows of the cache, and every token
         attends to the cache's positions up to its own -- the chunks before it and its own chunk's earlier tokens
         -- through the fused attention kernel reading keys and values where the cache holds them (whole 128-row
-        tiles: start and seq multiples of 128)."""
+        tiles: start and seq multiples of 128).
+        With a `LlamaPagedDecode` as the cache the prompts may be of several lengths (`lengths`, each 1 .. seq; the ids behind
+        a prompt's end are padding) and go to any of its sequences (`slots`, by default 0, 1, ..): rotation and cache write are
+        one op a layer (`rope_append_pages`), padding rows leave the cache as it is, and the logits are those of each prompt's
+        last token.  `cache.begin(slots, argmax, lengths)` then goes on from the prompts."""
         e, c, K = self.eng, self.cfg, kinds
         n = self.batch * self.seq
         chunked = start > 0
+        paged = isinstance(cache, LlamaPagedDecode)
+        if paged:
+            if chunked or cache.cfg is not self.cfg:
+                raise ValueError("a paged cache takes whole prompts of its own model")
+            lengths = [self.seq] * self.batch if lengths is None else [int(x) for x in lengths]
+            slots = list(range(self.batch)) if slots is None else [int(x) for x in slots]
+            if len(lengths) != self.batch or len(slots) != self.batch or len(set(slots)) != self.batch or not all(
+                    1 <= x <= self.seq for x in lengths) or not all(0 <= s < cache.batch for s in slots):
+                raise ValueError("a paged prefill takes a length of 1 .. seq and a sequence of its own for each prompt")
+            for s, x in zip(slots, lengths):
+                cache.reserve(s, x)
+            place = np.where(np.arange(self.seq)[None, :] < np.array(lengths)[:, None], np.arange(self.seq)[None, :], -1)
+            place = e.upload_bits(place.astype(np.int32).reshape(1, -1).view(np.uint32), 1, n, I32)
+            owner = e.upload_bits(np.repeat(np.array(slots, np.int32), self.seq).reshape(1, -1).view(np.uint32), 1, n, I32)
+        elif lengths is not None or slots is not None:
+            raise ValueError("prompts of several lengths need a paged cache")
         if chunked:
             if cache is None or not self.fused or start % 128:
                 raise ValueError("a later chunk needs a cache, the fused attention kernel and a start in whole 128-position tiles")
-        if cache is not None:
+        if cache is not None and not paged:
             assert cache.batch == self.batch and cache.max_len >= start + self.seq and cache.cfg is self.cfg
             key = (cache.max_len, start)
             if getattr(self, "_cache_rows_key", None) != key:
@@ -279,7 +310,13 @@ class LlamaPrefill:
             # RoPE on the query and key heads together: they share the head width and the tables (rope.rs:129)
             cos_b = (cache.cos, (start, 0), (t, hd)) if chunked else (self.cos, (0, 0), (t, hd))
             sin_b = (cache.sin, (start, 0), (t, hd)) if chunked else (self.sin, (0, 0), (t, hd))
-            if self.fused_rope:   # the rotation in the projection's own epilogue: the same bits, one launch less
+            if paged:             # rotation and cache write as one op; the rotated heads come back for the prompt's own attention
+                qkv, _ = e.matmul_dram_bf16(n1, False, self.w[f"l{l}.qkv"], False)
+                e.free(n1)
+                lab("rope + cache write")
+                qk, _ = e.rope_append_pages(cache.pages_shape, (qkv, (0, 0), (n, qk_cols + self.kv_cols)), self.cos, self.sin, place, owner,
+                                            cache.table, cache.kc[l], cache.vc[l], keys=True, bf16=True)
+            elif self.fused_rope:   # the rotation in the projection's own epilogue: the same bits, one launch less
                 qkv, _ = e.matmul_rope(n1, self.w[f"l{l}.qkv"], cos_b, sin_b, qk_cols)
                 e.free(n1)
                 qk = qkv          # the rotated query and key heads are the buffer's first columns
@@ -288,7 +325,7 @@ class LlamaPrefill:
                 e.free(n1)
                 lab("rope")
                 qk, _ = e.rope_blocks((qkv, (0, 0), (n, qk_cols)), cos_b, sin_b, hd, True)
-            if cache is not None:
+            if cache is not None and not paged:
                 lab("cache write")   # the chunk's rows of the cache: keys after RoPE, values as projected
                 e.scatter_rows_into(cache.kc[l], self._cache_rows, (qk, (0, self.q_cols), (n, self.kv_cols)))
                 e.scatter_rows_into(cache.vc[l], self._cache_rows, (qkv, (0, qk_cols), (n, self.kv_cols)))
@@ -354,13 +391,16 @@ class LlamaPrefill:
         if all_positions:
             last = x
         else:
-            last, _ = e.gather_rows([x], self.last_rows, c.hidden)           # last position only (llama.rs:1055-1061)
+            rows = [(0, b * t + lengths[b] - 1) for b in range(self.batch)] if paged else self.last_rows
+            last, _ = e.gather_rows([x], rows, c.hidden)                     # last position only (llama.rs:1055-1061)
             e.free(x)
         fn, _ = e.rms_norm_as(last, self.w["final_norm"], c.eps, True)
         e.free(last)
         logits, _ = e.matmul_dram(fn, False, self.w["embed"], True)          # tied head: last . table^T (llama.rs:1090)
         e.free(fn)
         am, _ = e.argmax_row(logits)                                         # generate::argmax
+        if paged:
+            e.free(place); e.free(owner)
         lab("")
         return logits, am
 
@@ -712,3 +752,159 @@ class LlamaDecode:
     def generated(self, first: int, count: int) -> np.ndarray:
         """The tokens recorded at positions first .. first + count - 1: [count, batch] I32."""
         return self.eng.download_bits(self.tokens).view(np.int32)[first:first + count]
+
+
+class LlamaPagedDecode:
+    """Generation of sequences of different lengths over a shared pool of cache pages: `batch` slots, each idle or a sequence
+    at its own position.  What `LlamaDecode` does for sequences in lockstep -- the same model, steps and roundings -- with a
+    layer's rotation and cache write as one op (`rope_append_pages`), attention over each slot's own pages
+    (`attention_pages`), and each step's choice with its log probability, the entropy and the `top` largest alternatives
+    (`token_logprobs`).  Positions, tokens and the page table are device tensors, so a captured step serves every position as
+    long as the pages it reaches are reserved; the pool's bookkeeping is the host's.
+
+    `weights_dev`: the device weights of a `LlamaPrefill` (shared, not copied)."""
+
+    def __init__(self, eng, cfg: LlamaConfig, weights_dev: Dict[str, int], batch: int, max_len: int, pages: int, page_size: int = 16, top: int = 0):
+        from .engine import PageShape
+        self.eng, self.cfg, self.w, self.batch, self.max_len, self.top = eng, cfg, weights_dev, batch, max_len, top
+        self.page_size, self.q_cols, self.kv_cols = page_size, cfg.heads * cfg.head_dim, cfg.kv_heads * cfg.head_dim
+        self.pages_shape = PageShape(cfg.heads, cfg.kv_heads, cfg.head_dim, page_size)
+        cos, sin = rope_tables(max_len, cfg.head_dim, cfg.theta)
+        self.cos, self.sin = eng.upload(cos, *cos.shape), eng.upload(sin, *sin.shape)
+        z = lambda: eng.zeros_dram((pages * page_size, self.kv_cols), bf16=True)[0]
+        self.kc = [z() for _ in range(cfg.layers)]
+        self.vc = [z() for _ in range(cfg.layers)]
+        self.spare = list(range(pages - 1, -1, -1))                      # pages no sequence holds
+        self.tables = np.full((batch, -(-max_len // page_size)), -1, np.int32)
+        self.lengths = np.full(batch, -1, np.int64)                      # a slot's position, -1: idle
+        i32 = lambda a, r, k: eng.upload_bits(np.ascontiguousarray(a, dtype=np.int32).view(np.uint32), r, k, I32)
+        self.table = i32(self.tables, *self.tables.shape)
+        self.pos, self.ids = i32(self.lengths, batch, 1), i32(np.zeros(batch), batch, 1)
+        self.trace = None
+
+    def reserve(self, slot: int, length: int):
+        """Pages for positions 0 .. length - 1 of a slot; MemoryError (and nothing taken) when the pool has not that many."""
+        if length > self.max_len:
+            raise ValueError(f"{length} positions and a cache of {self.max_len}")
+        need = -(-length // self.page_size)
+        have = int((self.tables[slot] >= 0).sum())
+        if need - have > len(self.spare):
+            raise MemoryError(f"{need - have} pages wanted, {len(self.spare)} spare")
+        if need > have:
+            for k in range(have, need):
+                self.tables[slot, k] = self.spare.pop()
+            self._push()
+
+    def _push(self):
+        self.eng.write_ptr(self.table, self.tables.ctypes.data, self.tables.size)
+
+    def _set(self, buf: int, slots, values):
+        """values[i] (a [n, 1] I32 buffer or a list) into the rows `slots` of a [batch, 1] buffer."""
+        e, n = self.eng, len(slots)
+        i32 = lambda a, r, k: e.upload_bits(np.ascontiguousarray(a, dtype=np.int32).view(np.uint32), r, k, I32)
+        rows = i32(slots, 1, n)
+        v = values if isinstance(values, int) else i32(values, n, 1)
+        e.scatter_rows_into(buf, rows, (v, (0, 0), (n, 1)))
+        e.free(rows)
+        if v is not values:
+            e.free(v)
+
+    def begin(self, slots, ids, positions):
+        """Slots go on (or start) at `positions` with `ids` (a list, or a [n, 1] I32 buffer: a prefill's argmax) as their next
+        input.  The cache holds their earlier positions already (a prefill wrote them), or the position is 0."""
+        self._set(self.ids, slots, ids)
+        self._set(self.pos, slots, list(positions))
+        self.lengths[list(slots)] = list(positions)
+
+    def finish(self, slot: int):
+        """The slot becomes idle and its pages go back to the pool."""
+        held = self.tables[slot][self.tables[slot] >= 0]
+        self.spare.extend(int(p) for p in held[::-1])
+        self.tables[slot] = -1
+        self.lengths[slot] = -1
+        self._push()
+        self._set(self.pos, [slot], [-1])
+
+    def _reserve_step(self):
+        for s in np.nonzero(self.lengths >= 0)[0]:
+            self.reserve(int(s), int(self.lengths[s]) + 1)
+
+    def _advance(self):
+        self.lengths[self.lengths >= 0] += 1
+
+    def step(self):
+        """One token for every live slot.  Returns {"logits" [batch, vocab], "argmax" [batch, 1] I32, "logprob", "entropy"
+        [batch, 1] and, with `top`, "top_ids", "top_logprobs" [batch, top]} buffers, which the caller frees; the rows of idle
+        slots mean nothing.  Advances the live slots' positions and feeds the argmax back."""
+        self._reserve_step()
+        out = self._step()
+        self._advance()
+        return out
+
+    def _step(self):
+        e, c, K, B, hd = self.eng, self.cfg, kinds, self.batch, self.cfg.head_dim
+        op = lambda kind, a, b=None, s1=0.0: e.eltwise_op(EltwiseOp(kind, s1, 0.0), a, b)[0]
+        emb, _ = e.select_rows(self.w["embed"], self.ids)
+        x, _ = e.cast_float(emb, False)
+        e.free(emb)
+        n1, _ = e.rms_norm_as(x, self.w["l0.norm1"], c.eps, True)
+        scale = 1.0 / float(np.sqrt(hd))
+        for l in range(c.layers):
+            qkv, _ = e.matmul_dram_bf16(n1, False, self.w[f"l{l}.qkv"], False)
+            e.free(n1)
+            # the queries stay F32, the keys are rounded once to BF16 as they are written (`LlamaDecode.step`)
+            q, _ = e.rope_append_pages(self.pages_shape, (qkv, (0, 0), (B, self.q_cols + 2 * self.kv_cols)), self.cos, self.sin, self.pos, None,
+                                       self.table, self.kc[l], self.vc[l])
+            e.free(qkv)
+            att, _ = e.attention_pages(self.pages_shape, (q, (0, 0), (B, self.q_cols)), self.kc[l], self.vc[l], self.table, self.pos, scale, bf16=True)
+            e.free(q)
+            o, _ = e.matmul_dram(att, False, self.w[f"l{l}.o"], False)
+            e.free(att)
+            (x2, _), (n2, _) = e.add_rms_norm_as(x, o, self.w[f"l{l}.norm2"], c.eps, True)
+            e.free(x); e.free(o)
+            gu, _ = e.matmul_dram_bf16(n2, False, self.w[f"l{l}.gate_up"], False)
+            e.free(n2)
+            act, _ = e.eltwise_blocks_as(EltwiseOp(K.SILU_MUL, 0.0, 0.0), (gu, (0, 0), (B, c.ff)), (gu, (0, c.ff), (B, c.ff)), None, True)
+            e.free(gu)
+            d, _ = e.matmul_dram(act, False, self.w[f"l{l}.down"], False)
+            e.free(act)
+            nxt = self.w[f"l{l + 1}.norm1"] if l + 1 < c.layers else self.w["final_norm"]
+            (x, _), (n1, _) = e.add_rms_norm_as(x2, d, nxt, c.eps, True)
+            e.free(x2); e.free(d)
+        e.free(x)
+        logits, _ = e.matmul_dram(n1, False, self.w["embed"], True)          # tied head
+        e.free(n1)
+        am, _ = e.argmax_row(logits)
+        scored = [i for i, _ in e.token_logprobs(logits, am, 1.0, self.top)]
+        e.free(scored[2])
+        e.copy_into(am, self.ids)
+        live = op(K.INT_GE_S, self.pos)
+        one = op(K.BOOL_TO_I32, live)
+        nxt_pos = op(K.INT_ADD, self.pos, one)                               # idle slots stay at -1
+        e.copy_into(nxt_pos, self.pos)
+        for i in (live, one, nxt_pos):
+            e.free(i)
+        out = {"logits": logits, "argmax": am, "logprob": scored[0], "entropy": scored[1]}
+        if self.top:
+            out.update(top_ids=scored[3], top_logprobs=scored[4])
+        return out
+
+    def capture(self):
+        """One eager step (so that every kernel is loaded) whose positions are put back, then the step captured.  Returns the
+        buffers a replay rewrites; `replay` runs one more step."""
+        e = self.eng
+        keep_pos, keep_ids = (e.eltwise_op(EltwiseOp(kinds.INT_ADD_S, 0.0, 0.0), b, None)[0] for b in (self.pos, self.ids))
+        self._reserve_step()
+        for i in self._step().values():
+            e.free(i)
+        e.copy_into(keep_pos, self.pos); e.copy_into(keep_ids, self.ids)
+        e.free(keep_pos); e.free(keep_ids)
+        e.begin_trace()
+        out = self._step()
+        self.trace = e.end_trace()
+        return out
+
+    def replay(self):
+        self._reserve_step()
+        self.eng.run_trace(self.trace)
+        self._advance()
