@@ -79,7 +79,7 @@ int page_view(b200_engine* e, const b200_page_shape* shape, b200_buffer key_page
                    shape->head_dim, shape->page_size);
   if ((K->elem != B200_F32 && K->elem != B200_BF16) || V->elem != K->elem)
     return e->fail(B200_UNSUPPORTED, "%s: key and value pages are both F32 or both BF16", what);
-  if (K->cols != width || V->cols != width || K->rows != V->rows || K->rows % shape->page_size || K->rows / shape->page_size > 0x7fffffffull)
+  if (K->cols != width || V->cols != width || K->rows != V->rows || K->rows % shape->page_size || K->rows > 0x7fffffffull)
     return e->fail(B200_UNSUPPORTED, "%s: key pages [%llu, %llu] and value pages [%llu, %llu] are not pages of %u rows of %llu columns", what,
                    (ull)K->rows, (ull)K->cols, (ull)V->rows, (ull)V->cols, shape->page_size, (ull)width);
   if ((reinterpret_cast<uintptr_t>(K->ptr) | reinterpret_cast<uintptr_t>(V->ptr)) & 15)
@@ -197,7 +197,14 @@ int32_t b200_attention_pages(b200_engine* e, const b200_page_shape* shape, const
   if (st) return st;
   g.positions = (const int32_t*)P->ptr;
   g.n = n; g.window = window; g.scale = scale; g.out = r.ptr; g.out_bf16 = out_bf16 ? 1 : 0; g.err = e->d_err;
-  st = e->launched(launch_attention_pages(g, e->stream), what, n ? 1 : 0);
+  int launches = 0;
+  void* scratch = nullptr;
+  uint64_t got = 0;
+  st = n ? e->alloc(attention_pages_scratch_bytes(shape->head_dim), &scratch, &got) : B200_OK;
+  if (st) { undo(e, r); return st; }
+  const cudaError_t ce = launch_attention_pages(g, scratch, &launches, e->stream);
+  if (n) e->release(scratch, got);
+  st = e->launched(ce, what, launches);
   if (st) { undo(e, r); return st; }
   *out = r.id;
   set_dims(out_dims, n, cols);
