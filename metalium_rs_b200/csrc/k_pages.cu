@@ -34,37 +34,148 @@ __device__ __forceinline__ int64_t pool_row(const PageView& c, uint32_t s, uint3
   return (int64_t)page * c.page + p % c.page;
 }
 
-// ---- append: a block a token.  x cos + swap(x) sin with the two products and the sum each rounded (`rope_blocks`' steps).
-__global__ void __launch_bounds__(128) rope_append_kernel(AppendArgs g) {
+// ---- append ---------------------------------------------------------------------
+// x cos + swap(x) sin with the two products and the sum each rounded (`rope_blocks`' steps).  Memory-bound: every element of
+// the projection is read once and written once or twice.
+
+// Token i's row of the pools; -1 for a padding row, and (with DOMAIN set) for a position or sequence outside its table.
+__device__ __forceinline__ int64_t token_row(const AppendArgs& g, uint64_t i, int32_t p) {
+  const int64_t s = g.sequences ? (int64_t)g.sequences[i] : (int64_t)i;
+  if (p == -1) return -1;
+  if (p < 0 || s < 0 || s >= g.cache.sequences || (uint64_t)p >= (uint64_t)g.cache.width * g.cache.page || (g.rotary && (uint64_t)p >= g.table_rows)) {
+    set_domain(g.err);
+    return -1;
+  }
+  return pool_row(g.cache, (uint32_t)s, (uint32_t)p, g.err);
+}
+
+struct Eight { float f[8]; };
+__device__ __forceinline__ Eight load8(const void* p, uint64_t i, int bf16) {
+  Eight v;
+  if (bf16) {
+    const uint4 w = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p) + i);
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) { v.f[2 * e] = __uint_as_float(u[e] << 16); v.f[2 * e + 1] = __uint_as_float(u[e] & 0xffff0000u); }
+  } else {
+    const float4* q = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p) + i);
+    const float4 a = q[0], b = q[1];
+    v.f[0] = a.x; v.f[1] = a.y; v.f[2] = a.z; v.f[3] = a.w; v.f[4] = b.x; v.f[5] = b.y; v.f[6] = b.z; v.f[7] = b.w;
+  }
+  return v;
+}
+// Two values as BF16, `f32_to_bf16_bits` of each: the hardware's conversion where that is the same rounding (a zero, or at least
+// 2^-126 in magnitude and not a NaN).
+__device__ __forceinline__ uint32_t narrow2(float lo, float hi) {
+  const uint32_t a = __float_as_uint(lo) & 0x7fffffffu, b = __float_as_uint(hi) & 0x7fffffffu;
+  uint32_t w;
+  if (min(a - 1u, b - 1u) < 0x007fffffu || max(a, b) > 0x7f800000u)
+    return (uint32_t)f32_to_bf16_bits(__float_as_uint(lo)) | ((uint32_t)f32_to_bf16_bits(__float_as_uint(hi)) << 16);
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(hi), "f"(lo));
+  return w;
+}
+__device__ __forceinline__ void store8(void* p, uint64_t i, int bf16, const Eight& v) {
+  if (bf16) {
+    *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(p) + i) =
+        make_uint4(narrow2(v.f[0], v.f[1]), narrow2(v.f[2], v.f[3]), narrow2(v.f[4], v.f[5]), narrow2(v.f[6], v.f[7]));
+  } else {
+    float4* q = reinterpret_cast<float4*>(reinterpret_cast<float*>(p) + i);
+    q[0] = make_float4(v.f[0], v.f[1], v.f[2], v.f[3]);
+    q[1] = make_float4(v.f[4], v.f[5], v.f[6], v.f[7]);
+  }
+}
+
+// Values that are only moved keep their bits where both sides are of one type.
+__device__ __forceinline__ void move8(void* to, uint64_t j, int to_bf16, const void* from, uint64_t i, int from_bf16) {
+  if (to_bf16 && from_bf16)
+    *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(to) + j) = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(from) + i);
+  else store8(to, j, to_bf16, load8(from, i, from_bf16));
+}
+__device__ __forceinline__ void move1(void* to, uint64_t j, int to_bf16, const void* from, uint64_t i, int from_bf16) {
+  if (to_bf16 && from_bf16) reinterpret_cast<uint16_t*>(to)[j] = reinterpret_cast<const uint16_t*>(from)[i];
+  else store_float(to, j, to_bf16, load_float(from, i, from_bf16));
+}
+
+// A block a token, eight columns a thread: thread (x, y) takes columns 8x of the low half of a rotation and the eight across from
+// them -- or, behind the rotation, eight columns that stay -- in heads y, y + blockDim.y, ..., so that its cos and sin entries are
+// read once for all of its heads (read again for every head they were twice the projection's bytes).
+__global__ void __launch_bounds__(512) rope_append_kernel(const __grid_constant__ AppendArgs g) {
   pdl_enter();
   const uint64_t i = blockIdx.x;
   const PageView& c = g.cache;
+  const uint32_t d = c.dim, half = g.rotary / 2, pairs = half / 8, turned = c.heads + c.kv_heads;
+  const uint32_t kept = c.heads + (g.keys_out ? c.kv_heads : 0), threads = blockDim.x * blockDim.y;
+  const uint32_t tid = threadIdx.y * blockDim.x + threadIdx.x;
+  const bool pair = threadIdx.x < pairs;
+  const uint32_t e0 = pair ? threadIdx.x * 8 : g.rotary + (threadIdx.x - pairs) * 8;
+  const uint64_t from = i * g.qkv.ld, to = i * (uint64_t)kept * d;
   const int32_t p = g.positions[i];
-  const int64_t s = g.sequences ? (int64_t)g.sequences[i] : (int64_t)i;
-  const uint32_t q_cols = c.heads * c.dim, kv_cols = c.kv_heads * c.dim;
+  const int64_t row = token_row(g, i, p);
+  if (row < 0) {
+    const Eight zero = {{0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}};
+    for (uint32_t j = tid; j < kept * d / 8; j += threads) store8(g.out, to + j * 8, g.out_bf16, zero);
+    return;
+  }
+  const uint64_t kv_cols = (uint64_t)c.kv_heads * d, at = (uint64_t)row * kv_cols;
+  if (pair) {
+    const uint64_t w = (uint64_t)p * g.rotary;
+    const Eight c0 = load8(g.cos, w + e0, 0), c1 = load8(g.cos, w + half + e0, 0), s0 = load8(g.sin, w + e0, 0), s1 = load8(g.sin, w + half + e0, 0);
+    for (uint32_t h = threadIdx.y; h < turned; h += blockDim.y) {
+      const Eight a = load8(g.qkv.p, from + (uint64_t)h * d + e0, g.qkv.bf16), b = load8(g.qkv.p, from + (uint64_t)h * d + half + e0, g.qkv.bf16);
+      Eight lo, hi;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        lo.f[e] = __fadd_rn(__fmul_rn(a.f[e], c0.f[e]), __fmul_rn(b.f[e], s0.f[e]));
+        hi.f[e] = __fadd_rn(__fmul_rn(b.f[e], c1.f[e]), __fmul_rn(a.f[e], s1.f[e]));
+      }
+      if (h < kept) {
+        store8(g.out, to + (uint64_t)h * d + e0, g.out_bf16, lo);
+        store8(g.out, to + (uint64_t)h * d + half + e0, g.out_bf16, hi);
+      }
+      if (h >= c.heads) {
+        store8(c.keys, at + (uint64_t)(h - c.heads) * d + e0, c.bf16, lo);
+        store8(c.keys, at + (uint64_t)(h - c.heads) * d + half + e0, c.bf16, hi);
+      }
+    }
+  } else {
+    for (uint32_t h = threadIdx.y; h < turned; h += blockDim.y) {
+      const uint64_t x = from + (uint64_t)h * d + e0;
+      if (h < kept) move8(g.out, to + (uint64_t)h * d + e0, g.out_bf16, g.qkv.p, x, g.qkv.bf16);
+      if (h >= c.heads) move8(c.keys, at + (uint64_t)(h - c.heads) * d + e0, c.bf16, g.qkv.p, x, g.qkv.bf16);
+    }
+  }
+  for (uint32_t j = tid; j < kv_cols / 8; j += threads)
+    move8(c.values, at + j * 8, c.bf16, g.qkv.p, from + (uint64_t)turned * d + j * 8, g.qkv.bf16);
+}
+
+// Blocks that start at no 16-byte address, and heads or rotations that are not groups of eight columns: an element a thread.
+__global__ void __launch_bounds__(128) rope_append_any_kernel(const __grid_constant__ AppendArgs g) {
+  pdl_enter();
+  const uint64_t i = blockIdx.x;
+  const PageView& c = g.cache;
+  const uint32_t q_cols = c.heads * c.dim, kv_cols = c.kv_heads * c.dim, half = g.rotary / 2;
   const uint32_t kept = q_cols + (g.keys_out ? kv_cols : 0);
-  int64_t row = -1;
-  if (p >= 0) {
-    if (s < 0 || s >= c.sequences || (uint64_t)p >= (uint64_t)c.width * c.page || (g.rotary && (uint64_t)p >= g.table_rows)) set_domain(g.err);
-    else row = pool_row(c, (uint32_t)s, (uint32_t)p, g.err);
-  } else if (p < -1) set_domain(g.err);
+  const int32_t p = g.positions[i];
+  const int64_t row = token_row(g, i, p);
   if (row < 0) {
     for (uint32_t j = threadIdx.x; j < kept; j += blockDim.x) store_float(g.out, i * kept + j, g.out_bf16, 0.f);
     return;
   }
-  const uint32_t half = g.rotary / 2;
   for (uint32_t j = threadIdx.x; j < q_cols + kv_cols; j += blockDim.x) {
     const uint32_t e = j % c.dim;
-    float v = load_float(g.qkv.p, i * g.qkv.ld + j, g.qkv.bf16);
-    if (e < g.rotary) {
+    if (e >= g.rotary) {
+      if (j < kept) move1(g.out, i * kept + j, g.out_bf16, g.qkv.p, i * g.qkv.ld + j, g.qkv.bf16);
+      if (j >= q_cols) move1(c.keys, (uint64_t)row * kv_cols + (j - q_cols), c.bf16, g.qkv.p, i * g.qkv.ld + j, g.qkv.bf16);
+    } else {
+      float v = load_float(g.qkv.p, i * g.qkv.ld + j, g.qkv.bf16);
       const float w = load_float(g.qkv.p, i * g.qkv.ld + (e < half ? j + half : j - half), g.qkv.bf16);
       v = __fadd_rn(__fmul_rn(v, g.cos[(uint64_t)p * g.rotary + e]), __fmul_rn(w, g.sin[(uint64_t)p * g.rotary + e]));
+      if (j < kept) store_float(g.out, i * kept + j, g.out_bf16, v);
+      if (j >= q_cols) store_float(c.keys, (uint64_t)row * kv_cols + (j - q_cols), c.bf16, v);
     }
-    if (j < kept) store_float(g.out, i * kept + j, g.out_bf16, v);
-    if (j >= q_cols) store_float(c.keys, (uint64_t)row * kv_cols + (j - q_cols), c.bf16, v);
   }
   for (uint32_t j = threadIdx.x; j < kv_cols; j += blockDim.x)
-    store_float(c.values, (uint64_t)row * kv_cols + j, c.bf16, load_float(g.qkv.p, i * g.qkv.ld + q_cols + kv_cols + j, g.qkv.bf16));
+    move1(c.values, (uint64_t)row * kv_cols + j, c.bf16, g.qkv.p, i * g.qkv.ld + q_cols + kv_cols + j, g.qkv.bf16);
 }
 
 // ---- attention ------------------------------------------------------------------
@@ -693,7 +804,18 @@ cudaError_t attention_form(const AttnPagesArgs& g, int sms, const AttnScratch& s
 
 cudaError_t launch_rope_append_pages(const AppendArgs& g, cudaStream_t stream) {
   if (g.n == 0) return cudaSuccess;
-  launch_pdl(rope_append_kernel, dim3((unsigned)g.n), dim3(128), 0, stream, g);
+  const uint32_t d = g.cache.dim, lanes = g.rotary / 16 + (d - g.rotary) / 8;   // of a head: pairs of eight columns, then eights
+  const uintptr_t ends = reinterpret_cast<uintptr_t>(g.qkv.p) | reinterpret_cast<uintptr_t>(g.cos) | reinterpret_cast<uintptr_t>(g.sin) |
+                         g.qkv.ld * (g.qkv.bf16 ? 2 : 4);
+  if (ends % 16 == 0 && d % 8 == 0 && g.rotary % 16 == 0 && lanes <= 512) {
+    // few tokens: a thread for every piece, so that a token's chain of loads is short; many: a quarter of that, as many tokens at once
+    const uint32_t want = g.n <= 592 ? 512 : 128, heads = g.cache.heads + g.cache.kv_heads;
+    uint32_t y = want / lanes;
+    y = y < 1 ? 1 : (y > heads ? heads : y);
+    launch_pdl(rope_append_kernel, dim3((unsigned)g.n), dim3(lanes, y), 0, stream, g);
+  } else {
+    launch_pdl(rope_append_any_kernel, dim3((unsigned)g.n), dim3(128), 0, stream, g);
+  }
   return cudaGetLastError();
 }
 

@@ -169,6 +169,28 @@ def test_append_is_the_trait_s_ops(eng):
         eng.free(i)
 
 
+@pytest.mark.parametrize("d,r", [(64, 32), (20, 4)])
+def test_values_and_unrotated_columns_of_one_type_keep_their_bits(eng, d, r):
+    """Subnormals, signed zeros, infinities and NaN payloads pass as `scatter_rows_into` passes them."""
+    rng = np.random.default_rng(3)
+    n, heads, kv = 5, 2, 1
+    bits = rng.integers(0, 1 << 16, (n, (heads + 2 * kv) * d)).astype(np.uint16)
+    bits[0, -4:] = [0x0001, 0x8000, 0x7F81, 0xFF80]
+    ix = eng.upload_bf16(bits, *bits.shape)
+    ik, iv = (eng.zeros_dram((16, kv * d), bf16=True)[0] for _ in range(2))
+    one, none = np.ones((8, r), np.float32), np.zeros((8, r), np.float32)
+    ic, isn = eng.upload(one, 8, r), eng.upload(none, 8, r)
+    it, ip, iq = up_i32(eng, [[1, 0]], 1, 2), up_i32(eng, np.arange(n), 1, n), up_i32(eng, np.zeros(n), 1, n)
+    out, _ = eng.rope_append_pages(PageShape(heads, kv, d, 8), (ix, (0, 0), bits.shape), ic, isn, ip, iq, it, ik, iv, bf16=True)
+    got, k, v = (eng.download_bf16(i) for i in (out, ik, iv))
+    keep = np.arange(d) >= r
+    assert np.array_equal(v[8:8 + n], bits[:, -d:])
+    assert np.array_equal(k[8:8 + n][:, keep], bits[:, heads * d:(heads + 1) * d][:, keep])
+    assert np.array_equal(got.reshape(n, heads, d)[:, :, keep], bits[:, :heads * d].reshape(n, heads, d)[:, :, keep])
+    for i in (ix, ik, iv, ic, isn, it, ip, iq, out):
+        eng.free(i)
+
+
 @pytest.mark.parametrize("bad", ["position", "below", "sequence", "page", "negative page", "rotation"])
 def test_append_reports_a_bad_index_and_writes_nothing_for_it(fresh_eng, bad):
     e = fresh_eng
