@@ -43,6 +43,7 @@ SOURCES = {
     "k_bfp.cu": [],
     "k_decode.cu": [],
     "k_pages.cu": [],
+    "k_attention_pages.cu": [],
     "k_logprob.cu": [],
     "k_pool.cu": ["-fmad=false"],
     "k_scan_sort.cu": ["-fmad=false"],
