@@ -1,4 +1,24 @@
 // Attention of one new token a sequence over the pages of its cache (`b200_attention_pages`).
+//
+// out = softmax(scale q K^T) V over one sequence's positions, up to eight query heads of one key/value head together, so that
+// keys and values are read once for all of them.  The bound is that read: HBM.
+//
+// Split: the batch's positions are one list of tiles of 16, sequence after sequence, cut into equal runs whatever the lengths,
+// and a warp takes one run for one key/value head: the warps beside it take the same run for the other heads, so that a cache
+// row's heads are read together (a row is one piece of memory).  A run may end inside a sequence and the next one goes on
+// there: a warp writes the results of sequences that lie in its run whole, and (maximum, sum, rows) of the at most two that do
+// not, which a second kernel joins.  The lengths are on the device, so the list is made there, from a prefix sum.  After that
+// sum no warp waits for another.
+//
+// A warp's pipeline: it copies its 16 keys and 16 values of a tile to its own shared memory by 16-byte asynchronous copies, a
+// few tiles ahead (row addresses through the page table, fetched one tile before they are used), and keeps its own running
+// maximum, sum and rows.
+//
+// Precision: keys and values are the cache's own values.  The tensor cores' tile has sixteen rows, and a head takes two of
+// them: row r has an operand's leading part and row r + 8 the next one, so one product does both.  On the BF16 path an F32
+// query is three BF16 parts (exact) or, for a BF16 result, two (2^-16), and so is a probability; on the F32 path every operand
+// is two TF32 parts, of whose four products three are kept (2^-21).  For an F32 result a tile's products start from zero and are
+// added to the running rows in F32; else the tensor cores accumulate them.
 #include <cfloat>
 #include <cmath>
 #include <cstdint>
@@ -12,60 +32,42 @@
 namespace b200 {
 namespace {
 
-// out = softmax(scale q K^T) V over one sequence's positions, the query heads of one key/value head (up to 16, one
-// tensor-core row tile) together, so that keys and values are read once for all of them.  The bound is that read: HBM.
-//
-// Split: the work is a list of tiles (16 positions a warp) in the order sequence, key/value head, position, and every block
-// takes an equal run of it, whatever the lengths: a block's run may end inside a sequence and the next block's goes on there.
-// A run's pieces that are whole (sequence, head) results are written at once, the others as (maximum, sum, rows) for the
-// second kernel to join, at most two a block.  The lengths are on the device, so the list is made there, from a prefix sum.
-//
-// A warp's own pipeline: it copies its 16 keys and 16 values of each tile to shared memory by 16-byte asynchronous copies,
-// a few tiles ahead (row addresses through the page table, fetched one tile before they are used), and keeps its own
-// running maximum, sum and rows; the block's warps meet only at the end of a (sequence, head).  Copies run on across it.
-//
-// Precision: keys and values are the cache's own values.  On the BF16 path the operands that are F32 are handed to the BF16
-// tensor cores as sums of BF16 parts -- an F32 query as three (exact) or, for a BF16 result, two (2^-16), a probability as
-// three or two -- since the tensor cores idle while the cache is read.  On the F32 path every operand is two TF32 parts and
-// three products are kept (2^-21).  For an F32 result a tile's
-// products start from zero and are added to the running rows in F32.
 template <typename KV, int D>
 struct Form {
   static constexpr bool BF = sizeof(KV) == 2;
   static constexpr int WARPS = !BF && D > 128 ? 2 : 4;        // an F32 tile of a wide head is 33 KB a warp
   static constexpr int THREADS = WARPS * 32;
-  static constexpr int TILE = WARPS * 16;                     // positions a block's step
   // shared-memory row pitches that let eight rows (or the four position pairs of an F32 fragment) fall into distinct banks
   static constexpr int K_PITCH = D * (int)sizeof(KV) + (BF ? 16 : 32);
   static constexpr int V_PITCH = D * (int)sizeof(KV) + 16;
-  static constexpr int Q_PITCH = K_PITCH;
-  static constexpr int STAGE = 16 * (K_PITCH + V_PITCH);      // a warp's stage
+  static constexpr int STAGE = 16 * (K_PITCH + V_PITCH);      // a warp's tile
   // a copy instruction: LANES lanes a row (a whole 128-byte line where rows are whole lines), ROWS rows; a lane's rows of a
   // tile are REST, its pieces of a row PIECES
   static constexpr int CHUNKS = D * (int)sizeof(KV) / 16;     // 16-byte pieces of a row
   static constexpr int LANES = CHUNKS % 8 ? 4 : 8, ROWS = 32 / LANES, REST = 16 / ROWS, PIECES = CHUNKS / LANES;
-  static constexpr int BLOCKS = BF ? (D <= 64 ? 4 : (D <= 128 ? 2 : 1)) : (D <= 64 ? 2 : 1);
-  static constexpr int SLAB = 16, SLAB_PITCH = 24;            // columns of the rows merged at a time
-  static constexpr int ML = WARPS * 16 * 2 * 4;
-  // the queries' parts; the same bytes hold the merged columns once a piece's products are done
-  static __host__ __device__ int q_bytes(int parts) {
-    const int q = parts * 16 * Q_PITCH, slab = WARPS * 16 * SLAB_PITCH * 4;
-    return q > slab ? q : slab;
-  }
+#ifndef ATTN_BLOCKS_128
+#define ATTN_BLOCKS_128 2
+#endif
+#ifndef ATTN_BLOCKS_64
+#define ATTN_BLOCKS_64 3
+#endif
+  static constexpr int BLOCKS = BF ? (D <= 64 ? ATTN_BLOCKS_64 : (D <= 128 ? ATTN_BLOCKS_128 : 1)) : (D <= 64 ? 2 : 1);
   static __host__ __device__ int prefix_bytes(uint32_t n) { return (int)(((n + 1) * 4 + 127) / 128 * 128); }
 };
 constexpr uint32_t MAX_SEQUENCES = 512;  // a launch's; its prefix sums lie in shared memory
 constexpr int MAX_STAGES = 4;
+constexpr int HEADS = 8;                 // query heads a warp
 
 struct AttnPlan {
   AttnPagesArgs g;
   uint64_t page_magic;                   // p / page = p * magic >> (32 + page_shift), exact below 2^31
   uint32_t page_shift;
-  uint32_t group, row_tiles;             // query heads a key/value head, and their tiles of 16
+  uint32_t group, row_tiles;             // query heads a key/value head, and their tiles of HEADS
   uint32_t jobs;                         // kv_heads * row_tiles
+  uint32_t runs, slot;                   // runs the tiles are cut into; floats of a piece
   int stages;
   float scale_log2;
-  float* part;                           // [blocks][2][16][D + 2]: rows, then (maximum, sum) a row
+  float* part;                           // [runs][jobs][2] pieces: [rows][D], then (maximum, sum) a row in four floats
   uint32_t* prefix;                      // [n + 1], for the join
 };
 
@@ -85,13 +87,26 @@ __device__ __forceinline__ void ldmatrix4(uint32_t* r, uint32_t at) {
 __device__ __forceinline__ void ldmatrix4_t(uint32_t* r, uint32_t at) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
 }
-__device__ __forceinline__ void mma_bf16(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
-  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+// Shared-memory loads in the order they are written: left to itself the compiler asks for a whole tile's fragments at once and
+// spills.
+__device__ __forceinline__ float2 lds2(uint32_t at) {
+  float2 v;
+  asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(at) : "memory");
+  return v;
 }
-__device__ __forceinline__ void mma_tf32(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
+__device__ __forceinline__ float lds1(uint32_t at) {
+  float v;
+  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+  return v;
+}
+// a: (row r, first half of the inner index), (row r + 8, first), (r, second), (r + 8, second)
+__device__ __forceinline__ void mma_bf16(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_tf32(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ uint32_t tf32_of(float x) {
   uint32_t r;
@@ -111,15 +126,24 @@ __device__ __forceinline__ uint32_t bf16x2(float lo, float hi) {
 __device__ __forceinline__ float low_of(uint32_t w) { return __uint_as_float(w << 16); }
 __device__ __forceinline__ float high_of(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
 
-// The first tile of block c's run, and the block that a tile is in: runs of total / blocks tiles.
-__device__ __forceinline__ uint32_t run_start(uint32_t total, uint32_t c, uint32_t blocks) { return total / blocks * c + total % blocks * c / blocks; }
-__device__ __forceinline__ uint32_t run_owner(uint32_t total, uint32_t tile, uint32_t blocks) {
-  uint32_t lo = 0, hi = blocks - 1;      // the last c whose run starts at or before `tile`
-  while (lo < hi) {
-    const uint32_t mid = (lo + hi + 1) / 2;
-    if (run_start(total, mid, blocks) <= tile) lo = mid; else hi = mid - 1;
-  }
-  return lo;
+// The next BF16 part of `rest`, which keeps what is left: cut, so that each part leaves fewer bits of the same sign, but for the
+// last, which is rounded.
+__device__ __forceinline__ uint32_t next_part(float& rest, bool last) {
+  uint32_t bits = __float_as_uint(rest);
+  if (last) bits = (uint32_t)f32_to_bf16_bits(bits) << 16;
+  else if (rest != rest) bits = 0x7fc00000u;
+  else bits &= 0xffff0000u;
+  const float part = __uint_as_float(bits);
+  rest = fabsf(part) <= FLT_MAX ? rest - part : 0.f;
+  return bits >> 16;
+}
+
+// The first tile of run c, and the run that a tile is in: runs of total / runs tiles.
+__device__ __forceinline__ uint32_t run_start(uint32_t total, uint32_t c, uint32_t runs) {
+  return total / runs * c + (uint32_t)((uint64_t)(total % runs) * c / runs);
+}
+__device__ __forceinline__ uint32_t run_owner(uint32_t total, uint32_t tile, uint32_t runs) {
+  return (uint32_t)((((uint64_t)tile + 1) * runs - 1) / total);
 }
 
 // A sequence's positions [lo, lo + count) that are attended to; a position outside the table (or below -1) sets DOMAIN.
@@ -133,16 +157,24 @@ __device__ __forceinline__ void span_of(const AttnPagesArgs& g, uint32_t s, uint
 
 // Where a warp's next tile lies.
 struct Cursor {
-  uint32_t s, job, tile, tiles, lo, end;
+  uint32_t s, tile, tiles, lo, end;
 };
 
-// QP: the queries' parts.  EXACT: an F32 result -- the weights in three parts, and every tile's products added to the rows in
-// F32; else two, the rows accumulated by the tensor cores and scaled only when a row's maximum moved.
+// The last sequence that starts at or before a tile of the list: it has tiles.
+__device__ __forceinline__ uint32_t sequence_of(const uint32_t* prefix, uint32_t n, uint32_t tile) {
+  uint32_t lo = 0, hi = n - 1;
+  while (lo < hi) {
+    const uint32_t mid = (lo + hi + 1) / 2;
+    if (prefix[mid] <= tile) lo = mid; else hi = mid - 1;
+  }
+  return lo;
+}
 
+// QP: the queries' parts.  EXACT: an F32 result.
 template <typename KV, int D, int QP, bool EXACT>
 __global__ void __launch_bounds__(Form<KV, D>::THREADS, Form<KV, D>::BLOCKS) attention_pages_kernel(const __grid_constant__ AttnPlan a) {
   using F = Form<KV, D>;
-  constexpr bool Q_HELD = F::BF && D <= 128 && QP * D <= 256;         // the queries' fragments stay in registers
+  constexpr int ROW_REGS = F::BF && !EXACT ? 4 : 2;       // accumulated by the tensor cores, both parts of a row are
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ uint32_t warp_sum[F::WARPS];
   __shared__ uint32_t valid[F::WARPS][MAX_STAGES];
@@ -150,12 +182,9 @@ __global__ void __launch_bounds__(Form<KV, D>::THREADS, Form<KV, D>::BLOCKS) att
   const AttnPagesArgs& g = a.g;
   const PageView& cache = g.cache;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const uint32_t n = (uint32_t)g.n, block = blockIdx.x, blocks = gridDim.x;
-  uint32_t* prefix = reinterpret_cast<uint32_t*>(smem);                       // [n + 1] tiles before a sequence, of all its jobs
-  float* ml = reinterpret_cast<float*>(smem + F::prefix_bytes(n));            // [warps][16] (maximum, sum)
-  unsigned char* q_sm = reinterpret_cast<unsigned char*>(ml) + F::ML;         // [parts][16] rows
-  float* slab = reinterpret_cast<float*>(q_sm);                               // [warps][16][SLAB_PITCH]
-  unsigned char* stages = q_sm + F::q_bytes(QP) + warp * a.stages * F::STAGE;
+  const uint32_t n = (uint32_t)g.n;
+  uint32_t* prefix = reinterpret_cast<uint32_t*>(smem);                       // [n + 1] tiles before a sequence
+  unsigned char* stages = smem + F::prefix_bytes(n) + warp * a.stages * F::STAGE;
 
   // ---- the tile list: a prefix sum over the sequences; rows of sequences without positions are zero
   {
@@ -165,7 +194,7 @@ __global__ void __launch_bounds__(Form<KV, D>::THREADS, Form<KV, D>::BLOCKS) att
       uint32_t lo, count;
       span_of(g, s, &lo, &count);
       prefix[s] = sum;
-      sum += (count + F::TILE - 1) / F::TILE * a.jobs;
+      sum += (count + 15) / 16;
     }
     uint32_t scan = sum;
 #pragma unroll
@@ -182,444 +211,378 @@ __global__ void __launch_bounds__(Form<KV, D>::THREADS, Form<KV, D>::BLOCKS) att
     __syncthreads();
   }
   const uint32_t total = prefix[n];
-  if (block == 0)
+  if (blockIdx.x == 0)
     for (uint32_t s = tid; s <= n; s += F::THREADS) a.prefix[s] = prefix[s];
   const uint32_t out_cols = cache.heads * D;
-  for (uint32_t s = block; s < n; s += blocks)
+  for (uint32_t s = blockIdx.x; s < n; s += gridDim.x)
     if (prefix[s] == prefix[s + 1])
       for (uint32_t j = tid; j < out_cols; j += F::THREADS) store_float(g.out, (uint64_t)s * out_cols + j, g.out_bf16, 0.f);
-  const uint32_t start = run_start(total, block, blocks), stop = run_start(total, block + 1, blocks);
-  if (start >= stop) return;             // the same for every thread
 
   const auto enter = [&](Cursor& c) {    // the bounds of sequence c.s
     uint32_t count;
     span_of(g, c.s, &c.lo, &count);
     c.end = c.lo + count;
-    c.tiles = (count + F::TILE - 1) / F::TILE;
+    c.tiles = (count + 15) / 16;
   };
   const auto seek = [&](Cursor& c, uint32_t tile) {
-    uint32_t lo = 0, hi = n - 1;         // the last sequence that starts at or before the tile: it has tiles
-    while (lo < hi) {
-      const uint32_t mid = (lo + hi + 1) / 2;
-      if (prefix[mid] <= tile) lo = mid; else hi = mid - 1;
-    }
-    c.s = lo;
+    c.s = sequence_of(prefix, n, tile);
     enter(c);
-    c.job = (tile - prefix[lo]) / c.tiles;
-    c.tile = (tile - prefix[lo]) % c.tiles;
+    c.tile = tile - prefix[c.s];
   };
-  const auto next_job = [&](Cursor& c) {
+  const auto next_sequence = [&](Cursor& c) {
     c.tile = 0;
-    if (++c.job == a.jobs) {
-      c.job = 0;
-      do ++c.s; while (c.s < n && prefix[c.s] == prefix[c.s + 1]);
-      if (c.s < n) enter(c);
-    }
+    do ++c.s; while (c.s < n && prefix[c.s] == prefix[c.s + 1]);
+    if (c.s < n) enter(c);
   };
-
-  // ---- the copies' side of the pipeline: rows of the tile that is issued next
-  Cursor ahead;
-  seek(ahead, start);
-  uint32_t to_issue = stop - start;
-  int32_t row = -1;                      // lane % 16's pool row of the tile at `ahead`, -1: not attended
-  const auto look_up = [&]() {
-    row = -1;
-    const uint32_t p = ahead.lo + ahead.tile * F::TILE + warp * 16 + (lane & 15);
-    if (to_issue && p < ahead.end) {
-      const uint32_t at = (uint32_t)(((uint64_t)p * a.page_magic) >> (32 + a.page_shift));
-      const int32_t page = cache.table[(uint64_t)ahead.s * cache.width + at];
-      if (page >= 0 && (uint32_t)page < cache.pages) row = page * (int32_t)cache.page + (int32_t)(p - at * cache.page);
-      else set_domain(g.err);
-    }
-  };
-  look_up();
-  const uint32_t ld = cache.kv_heads * D * (uint32_t)sizeof(KV);           // bytes of a pool row
-  uint32_t head_at = ahead.job / a.row_tiles * D * (uint32_t)sizeof(KV);   // of the head of the tile at `ahead`
-  const uint32_t to = (uint32_t)__cvta_generic_to_shared(stages) + (lane % F::LANES) * 16;
-  int issue_stage = 0;
-  const auto issue = [&]() {
-    if (to_issue) {
-      const uint32_t there = __ballot_sync(0xffffffffu, row >= 0);
-      if (lane == 0) valid[warp][issue_stage] = there & 0xffffu;
-      const uint32_t at = to + issue_stage * F::STAGE;
-#pragma unroll
-      for (int i = 0; i < F::REST; ++i) {
-        const int r = i * F::ROWS + lane / F::LANES;
-        const int32_t from = __shfl_sync(0xffffffffu, row, r);
-        const bool on = from >= 0;
-        const uint64_t off = (uint64_t)(uint32_t)(on ? from : 0) * ld + head_at + (lane % F::LANES) * 16;
-        const char *k = (const char*)cache.keys + off, *v = (const char*)cache.values + off;
-#pragma unroll
-        for (int c = 0; c < F::PIECES; ++c) {
-          cp_async16(at + r * F::K_PITCH + c * F::LANES * 16, k + c * F::LANES * 16, on);
-          cp_async16(at + 16 * F::K_PITCH + r * F::V_PITCH + c * F::LANES * 16, v + c * F::LANES * 16, on);
-        }
-      }
-      --to_issue;
-      if (++ahead.tile == ahead.tiles) {
-        next_job(ahead);
-        head_at = ahead.job / a.row_tiles * D * (uint32_t)sizeof(KV);
-      }
-      look_up();
-    }
-    cp_async_commit();
-    if (++issue_stage == a.stages) issue_stage = 0;
-  };
-  for (int i = 0; i + 1 < a.stages; ++i) issue();
-
-  // ---- the block's (sequence, head) pieces, one after another
-  Cursor here;
-  seek(here, start);
   const int gr = lane >> 2, t4 = lane & 3;
-  int stage = 0, piece_i = 0;
-  for (uint32_t left = stop - start; left > 0; ++piece_i) {
-    const uint32_t steps = left < here.tiles - here.tile ? left : here.tiles - here.tile;
-    const bool whole = here.tile == 0 && steps == here.tiles;
-    const uint32_t kvh = here.job / a.row_tiles, r0 = (here.job % a.row_tiles) * 16;
-    const uint32_t rows = a.group - r0 < 16 ? a.group - r0 : 16;             // query heads of this tile
-    const uint32_t head0 = kvh * a.group + r0;
+  const uint32_t ld = cache.kv_heads * D * (uint32_t)sizeof(KV);              // bytes of a pool row
+  const uint32_t to = (uint32_t)__cvta_generic_to_shared(stages) + (lane % F::LANES) * 16;
 
-    // the queries, in the parts the products take; rows without a head are zero
-    __syncthreads();                     // the last piece's readers are done
-    for (int i = tid; i < 16 * D; i += F::THREADS) {
-      const int r = i / D, e = i % D;
-      const float q = r < (int)rows ? load_float(g.q.p, (uint64_t)here.s * g.q.ld + (uint64_t)(head0 + r) * D + e, g.q.bf16) : 0.f;
-      if constexpr (F::BF) {
-        float rest = q;
-        for (int p = 0; p < QP; ++p) {
-          // all parts but the last are cut, so that each leaves fewer bits of the same sign; the last is rounded
-          uint32_t bits = __float_as_uint(rest);
-          if (p + 1 == QP) bits = (uint32_t)f32_to_bf16_bits(bits) << 16;
-          else if (rest != rest) bits = 0x7fc00000u;
-          else bits &= 0xffff0000u;
-          *reinterpret_cast<uint16_t*>(q_sm + (p * 16 + r) * F::Q_PITCH + e * 2) = (uint16_t)(bits >> 16);
-          const float part = __uint_as_float(bits);
-          rest = fabsf(part) <= FLT_MAX ? rest - part : 0.f;
-        }
-      } else {
-        const float hi = __uint_as_float(tf32_of(q));
-        *reinterpret_cast<float*>(q_sm + r * F::Q_PITCH + e * 4) = hi;
-        *reinterpret_cast<float*>(q_sm + (16 + r) * F::Q_PITCH + e * 4) = fabsf(hi) <= FLT_MAX ? q - hi : 0.f;
+  const uint32_t tasks = a.runs * a.jobs;
+  for (uint32_t task = blockIdx.x * F::WARPS + warp; task < tasks; task += gridDim.x * F::WARPS) {   // the same for a warp's lanes
+    const uint32_t run = task / a.jobs, job = task % a.jobs;
+    const uint32_t start = run_start(total, run, a.runs), stop = run_start(total, run + 1, a.runs);
+    if (start >= stop) continue;
+    const uint32_t kvh = job / a.row_tiles, r0 = job % a.row_tiles * HEADS;
+    const uint32_t rows = a.group - r0 < HEADS ? a.group - r0 : HEADS, head0 = kvh * a.group + r0;
+
+    // ---- the copies' side: the rows of the tile that is issued next
+    Cursor ahead;
+    seek(ahead, start);
+    uint32_t to_issue = stop - start;
+    int32_t row = -1;                    // lane % 16's pool row of the tile at `ahead`, -1: not attended
+    const auto look_up = [&]() {
+      row = -1;
+      const uint32_t p = ahead.lo + ahead.tile * 16 + (lane & 15);
+      if (to_issue && p < ahead.end) {
+        const uint32_t at = (uint32_t)(((uint64_t)p * a.page_magic) >> (32 + a.page_shift));
+        const int32_t page = cache.table[(uint64_t)ahead.s * cache.width + at];
+        if (page >= 0 && (uint32_t)page < cache.pages) row = page * (int32_t)cache.page + (int32_t)(p - at * cache.page);
+        else set_domain(g.err);
       }
-    }
-    __syncthreads();
-
-    uint32_t qf[Q_HELD ? QP : 1][Q_HELD ? D / 16 : 1][4];
-    if constexpr (Q_HELD) {
-      const uint32_t qa = (uint32_t)__cvta_generic_to_shared(q_sm) + ((lane & 7) + ((lane >> 3) & 1) * 8) * F::Q_PITCH + (lane >> 4) * 16;
+    };
+    look_up();
+    const uint64_t head_at = (uint64_t)kvh * D * sizeof(KV) + (lane % F::LANES) * 16;
+    const char *key_at = (const char*)cache.keys + head_at, *value_at = (const char*)cache.values + head_at;
+    int issue_stage = 0;
+    const auto issue = [&]() {
+      if (to_issue) {
+        const uint32_t there = __ballot_sync(0xffffffffu, row >= 0);
+        if (lane == 0) valid[warp][issue_stage] = there & 0xffffu;
+        const uint32_t at = to + issue_stage * F::STAGE;
 #pragma unroll
-      for (int p = 0; p < QP; ++p)
+        for (int i = 0; i < F::REST; ++i) {
+          const int r = i * F::ROWS + lane / F::LANES;
+          const int32_t from = __shfl_sync(0xffffffffu, row, r);
+          const bool on = from >= 0;
+          const uint64_t off = (uint64_t)(uint32_t)(on ? from : 0) * ld;
 #pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) ldmatrix4(qf[p][kk], qa + p * 16 * F::Q_PITCH + kk * 32);
-    }
-    float o[D / 8][4];
-#pragma unroll
-    for (int j = 0; j < D / 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
-    float m0 = -FLT_MAX, m1 = -FLT_MAX, l0 = 0.f, l1 = 0.f;      // rows gr and gr + 8; the sums are this lane's own
-    for (uint32_t step = 0; step < steps; ++step) {
-      cp_async_wait(a.stages - 2);
-      __syncwarp();                      // every lane's copies of this stage are in, and every lane is done with the stage before
-      issue();
-      const unsigned char* st = stages + stage * F::STAGE;
-      const uint32_t live = valid[warp][stage];
-      if (++stage == a.stages) stage = 0;
-      const uint32_t k_at = (uint32_t)__cvta_generic_to_shared(st), v_at = k_at + 16 * F::K_PITCH;
-      const uint32_t q_at = (uint32_t)__cvta_generic_to_shared(q_sm);
-
-      // scores of 16 heads x 16 positions: lane holds rows gr, gr + 8 and positions 8 nt + 2 t4 + {0, 1}
-      float sc[2][4];
-#pragma unroll
-      for (int nt = 0; nt < 2; ++nt) sc[nt][0] = sc[nt][1] = sc[nt][2] = sc[nt][3] = 0.f;
-      if constexpr (F::BF) {
-        const uint32_t kb = k_at + ((lane & 7) + ((lane >> 4) & 1) * 8) * F::K_PITCH + ((lane >> 3) & 1) * 16;
-        const uint32_t qa = q_at + ((lane & 7) + ((lane >> 3) & 1) * 8) * F::Q_PITCH + (lane >> 4) * 16;
-        float odd_k[2][4];               // two chains of products a score: each waits for the one before it
-#pragma unroll
-        for (int nt = 0; nt < 2; ++nt) odd_k[nt][0] = odd_k[nt][1] = odd_k[nt][2] = odd_k[nt][3] = 0.f;
-#pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) {
-          uint32_t b[4];
-          ldmatrix4(b, kb + kk * 32);
-          auto& to_sum = kk & 1 ? odd_k : sc;
-#pragma unroll
-          for (int p = 0; p < QP; ++p) {
-            if constexpr (Q_HELD) {
-              mma_bf16(to_sum[0], qf[p][kk], b[0], b[1]);
-              mma_bf16(to_sum[1], qf[p][kk], b[2], b[3]);
-            } else {
-              uint32_t x[4];
-              ldmatrix4(x, qa + p * 16 * F::Q_PITCH + kk * 32);
-              mma_bf16(to_sum[0], x, b[0], b[1]);
-              mma_bf16(to_sum[1], x, b[2], b[3]);
-            }
+          for (int c = 0; c < F::PIECES; ++c) {
+            cp_async16(at + r * F::K_PITCH + c * F::LANES * 16, key_at + off + c * F::LANES * 16, on);
+            cp_async16(at + 16 * F::K_PITCH + r * F::V_PITCH + c * F::LANES * 16, value_at + off + c * F::LANES * 16, on);
           }
         }
-#pragma unroll
-        for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) sc[nt][e] += odd_k[nt][e];
-      } else {
-        // the products' inner index in the order 0, 2, 4, 6, 1, 3, 5, 7 of each eight columns, for both operands
-        const float* qh = reinterpret_cast<const float*>(q_sm + gr * F::Q_PITCH) + 2 * t4;
-        constexpr int ROW8 = 8 * F::Q_PITCH / 4, LOW = 16 * F::Q_PITCH / 4;
-#pragma unroll 4
-        for (int kk = 0; kk < D / 8; ++kk) {
-          const float2 h0 = *reinterpret_cast<const float2*>(qh + kk * 8), h1 = *reinterpret_cast<const float2*>(qh + ROW8 + kk * 8);
-          const float2 w0 = *reinterpret_cast<const float2*>(qh + LOW + kk * 8), w1 = *reinterpret_cast<const float2*>(qh + LOW + ROW8 + kk * 8);
-          const uint32_t hi[4] = {__float_as_uint(h0.x), __float_as_uint(h1.x), __float_as_uint(h0.y), __float_as_uint(h1.y)};
-          const uint32_t lo[4] = {__float_as_uint(w0.x), __float_as_uint(w1.x), __float_as_uint(w0.y), __float_as_uint(w1.y)};
-#pragma unroll
-          for (int nt = 0; nt < 2; ++nt) {
-            const float2 k = *reinterpret_cast<const float2*>(st + (nt * 8 + gr) * F::K_PITCH + (kk * 8 + 2 * t4) * 4);
-            const uint32_t b0 = tf32_of(k.x), b1 = tf32_of(k.y);
-            mma_tf32(sc[nt], lo, b0, b1);
-            mma_tf32(sc[nt], hi, __float_as_uint(k.x - __uint_as_float(b0)), __float_as_uint(k.y - __uint_as_float(b1)));
-            mma_tf32(sc[nt], hi, b0, b1);
-          }
-        }
+        --to_issue;
+        if (++ahead.tile == ahead.tiles) next_sequence(ahead);
+        look_up();
       }
-      // An infinite key gives 0 * inf among the parts' products: such a score is taken again from whole operands.
-      bool odd = false;
+      cp_async_commit();
+      if (++issue_stage == a.stages) issue_stage = 0;
+    };
+    for (int i = 0; i + 1 < a.stages; ++i) issue();
+
+    // ---- the run's sequences, one after another
+    Cursor here;
+    seek(here, start);
+    int stage = 0, piece = 0;
+    for (uint32_t left = stop - start; left > 0; ++piece) {
+      const uint32_t steps = left < here.tiles - here.tile ? left : here.tiles - here.tile;
+      const bool whole = here.tile == 0 && steps == here.tiles;
+
+      // the queries' fragments: row gr's leading part and, as row gr + 8, its next one (the third by itself); on the F32 path
+      // the queries themselves, which a product takes apart (their parts are too many registers)
+      uint32_t qf[D / (F::BF ? 16 : 8)][F::BF ? 2 * QP : 2];
+      {
+        const uint64_t from = (uint64_t)here.s * g.q.ld + (uint64_t)(head0 + gr) * D;
+        const bool live = gr < (int)rows;
+        if constexpr (F::BF) {
 #pragma unroll
-      for (int nt = 0; nt < 2; ++nt)
+          for (int kk = 0; kk < D / 16; ++kk)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) odd |= sc[nt][e] != sc[nt][e];
-      if (__any_sync(0xffffffffu, odd)) {
+            for (int hf = 0; hf < 2; ++hf) {
+              const int e = kk * 16 + hf * 8 + 2 * t4;
+              float u = live ? load_float(g.q.p, from + e, g.q.bf16) : 0.f, v = live ? load_float(g.q.p, from + e + 1, g.q.bf16) : 0.f;
 #pragma unroll
-        for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (sc[nt][e] != sc[nt][e]) {
-              const int r = gr + (e >> 1) * 8, j = nt * 8 + 2 * t4 + (e & 1);
-              float t = 0.f;
-              for (int c = 0; c < D; ++c) {
-                float q = 0.f;
-                for (int p = 0; p < QP; ++p)
-                  q += F::BF ? bf16_bits_to_f32(*reinterpret_cast<const uint16_t*>(q_sm + (p * 16 + r) * F::Q_PITCH + c * 2))
-                             : *reinterpret_cast<const float*>(q_sm + (p * 16 + r) * F::Q_PITCH + c * 4);
-                t = fmaf(q, F::BF ? bf16_bits_to_f32(*reinterpret_cast<const uint16_t*>(st + j * F::K_PITCH + c * 2))
-                                  : *reinterpret_cast<const float*>(st + j * F::K_PITCH + c * 4), t);
+              for (int p = 0; p < QP; ++p) {
+                const uint32_t x = next_part(u, p + 1 == QP), y = next_part(v, p + 1 == QP);
+                qf[kk][p * 2 + hf] = x | (y << 16);
               }
-              sc[nt][e] = t;
             }
+        } else {
+          // the products' inner index in the order 0, 2, 4, 6, 1, 3, 5, 7 of each eight columns, for both operands
+#pragma unroll
+          for (int kk = 0; kk < D / 8; ++kk)
+#pragma unroll
+            for (int hf = 0; hf < 2; ++hf) {
+              qf[kk][hf] = live ? __float_as_uint(load_float(g.q.p, from + kk * 8 + 2 * t4 + hf, g.q.bf16)) : 0u;
+            }
+        }
       }
+      float o[D / 8][ROW_REGS];
+#pragma unroll
+      for (int j = 0; j < D / 8; ++j)
+#pragma unroll
+        for (int e = 0; e < ROW_REGS; ++e) o[j][e] = 0.f;
+      float m = -FLT_MAX, l = 0.f;       // row gr's; the sum is this lane's own
+      for (uint32_t step = 0; step < steps; ++step) {
+        cp_async_wait(a.stages - 2);
+        __syncwarp();                    // every lane's copies of this stage are in, and every lane is done with the stage before
+        issue();
+        const unsigned char* st = stages + stage * F::STAGE;
+        const uint32_t live = valid[warp][stage];
+        if (++stage == a.stages) stage = 0;
+        const uint32_t k_at = (uint32_t)__cvta_generic_to_shared(st), v_at = k_at + 16 * F::K_PITCH;
 
-      // running softmax: new maximum, the factor of what was summed before, the weights
-      float x0 = -FLT_MAX, x1 = -FLT_MAX;
+        // scores of 8 heads x 16 positions: lane holds row gr and positions 8 nt + 2 t4 + {0, 1}
+        float x[2][2];
+        if constexpr (F::BF) {
+          const uint32_t kb = k_at + ((lane & 7) + ((lane >> 4) & 1) * 8) * F::K_PITCH + ((lane >> 3) & 1) * 16;
+          float c[2][2][4];              // two chains of products a score: each waits for the one before it
 #pragma unroll
-      for (int nt = 0; nt < 2; ++nt)
+          for (int i = 0; i < 8; ++i) c[i >> 2][(i >> 1) & 1][(i & 1) * 2] = c[i >> 2][(i >> 1) & 1][(i & 1) * 2 + 1] = 0.f;
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const bool on = (live >> (nt * 8 + 2 * t4 + e)) & 1;
-          sc[nt][e] = on ? sc[nt][e] * a.scale_log2 : -INFINITY;
-          sc[nt][2 + e] = on ? sc[nt][2 + e] * a.scale_log2 : -INFINITY;
-          x0 = fmaxf(x0, sc[nt][e]);
-          x1 = fmaxf(x1, sc[nt][2 + e]);
-        }
-      x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, 1)); x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, 2));
-      x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, 1)); x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, 2));
-      x0 = fmaxf(x0, m0); x1 = fmaxf(x1, m1);
-      const float f0 = exp2_fast(m0 - x0), f1 = exp2_fast(m1 - x1);
-      m0 = x0; m1 = x1;
+          for (int kk = 0; kk < D / 16; ++kk) {
+            uint32_t b[4];
+            ldmatrix4(b, kb + kk * 32);
 #pragma unroll
-      for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          sc[nt][e] = exp2_fast(sc[nt][e] - m0);
-          sc[nt][2 + e] = exp2_fast(sc[nt][2 + e] - m1);
-        }
-      l0 = l0 * f0 + ((sc[0][0] + sc[0][1]) + (sc[1][0] + sc[1][1]));
-      l1 = l1 * f1 + ((sc[0][2] + sc[0][3]) + (sc[1][2] + sc[1][3]));
-
-      // rows = rows * factor + weights x values
-      if constexpr (F::BF) {
-        uint32_t w[3][4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {          // (row gr, first eight), (gr + 8, first), (gr, second), (gr + 8, second)
-          float u = sc[i >> 1][(i & 1) * 2], v = sc[i >> 1][(i & 1) * 2 + 1];
-          w[0][i] = bf16x2(u, v);
-          u -= low_of(w[0][i]); v -= high_of(w[0][i]);
-          w[1][i] = bf16x2(u, v);
-          if constexpr (EXACT) w[2][i] = bf16x2(u - low_of(w[1][i]), v - high_of(w[1][i]));
-        }
-        if constexpr (!EXACT)
-          if (__any_sync(0xffffffffu, f0 != 1.f || f1 != 1.f)) {
-#pragma unroll
-            for (int j = 0; j < D / 8; ++j) { o[j][0] *= f0; o[j][1] *= f0; o[j][2] *= f1; o[j][3] *= f1; }
-          }
-        const uint32_t vb = v_at + ((lane & 7) + ((lane >> 3) & 1) * 8) * F::V_PITCH + (lane >> 4) * 16;
-#pragma unroll
-        for (int j = 0; j < D / 16; ++j) {
-          uint32_t b[4];
-          ldmatrix4_t(b, vb + j * 32);
-#pragma unroll
-          for (int hf = 0; hf < 2; ++hf) {
-            float* r = o[2 * j + hf];
-            if constexpr (EXACT) {
-              float c[4] = {0.f, 0.f, 0.f, 0.f};
-              mma_bf16(c, w[2], b[2 * hf], b[2 * hf + 1]);
-              mma_bf16(c, w[1], b[2 * hf], b[2 * hf + 1]);
-              mma_bf16(c, w[0], b[2 * hf], b[2 * hf + 1]);
-              r[0] = fmaf(r[0], f0, c[0]); r[1] = fmaf(r[1], f0, c[1]);
-              r[2] = fmaf(r[2], f1, c[2]); r[3] = fmaf(r[3], f1, c[3]);
-            } else {
-              mma_bf16(r, w[1], b[2 * hf], b[2 * hf + 1]);
-              mma_bf16(r, w[0], b[2 * hf], b[2 * hf + 1]);
+            for (int nt = 0; nt < 2; ++nt) {
+              if constexpr (QP == 1) mma_bf16(c[kk & 1][nt], qf[kk][0], 0u, qf[kk][1], 0u, b[2 * nt], b[2 * nt + 1]);
+              else mma_bf16(c[kk & 1][nt], qf[kk][0], qf[kk][2], qf[kk][1], qf[kk][3], b[2 * nt], b[2 * nt + 1]);
+              if constexpr (QP == 3) mma_bf16(c[kk & 1][nt], 0u, qf[kk][4], 0u, qf[kk][5], b[2 * nt], b[2 * nt + 1]);
             }
           }
-        }
-      } else {
-        uint32_t hi[2][4], lo[2][4];
 #pragma unroll
-        for (int nt = 0; nt < 2; ++nt) {
-          const float v[4] = {sc[nt][0], sc[nt][2], sc[nt][1], sc[nt][3]};   // (gr, even), (gr + 8, even), (gr, odd), (gr + 8, odd)
+          for (int nt = 0; nt < 2; ++nt)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            hi[nt][i] = tf32_of(v[i]);
-            lo[nt][i] = __float_as_uint(v[i] - __uint_as_float(hi[nt][i]));
+            for (int e = 0; e < 2; ++e) {
+              x[nt][e] = c[0][nt][e] + c[1][nt][e];
+              if constexpr (QP > 1) x[nt][e] += c[0][nt][2 + e] + c[1][nt][2 + e];
+            }
+        } else {
+          float c[2][2][4];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) c[i >> 2][(i >> 1) & 1][(i & 1) * 2] = c[i >> 2][(i >> 1) & 1][(i & 1) * 2 + 1] = 0.f;
+#pragma unroll
+          for (int kk = 0; kk < D / 8; ++kk) {
+            const uint32_t q0 = tf32_of(__uint_as_float(qf[kk][0])), q1 = tf32_of(__uint_as_float(qf[kk][1]));
+            const uint32_t p0 = __float_as_uint(__uint_as_float(qf[kk][0]) - __uint_as_float(q0)), p1 = __float_as_uint(__uint_as_float(qf[kk][1]) - __uint_as_float(q1));
+#pragma unroll
+            for (int nt = 0; nt < 2; ++nt) {
+              const float2 k = lds2(k_at + (nt * 8 + gr) * F::K_PITCH + (kk * 8 + 2 * t4) * 4);
+              const uint32_t b0 = tf32_of(k.x), b1 = tf32_of(k.y);
+              mma_tf32(c[kk & 1][nt], q0, 0u, q1, 0u, __float_as_uint(k.x - __uint_as_float(b0)), __float_as_uint(k.y - __uint_as_float(b1)));
+              mma_tf32(c[kk & 1][nt], q0, p0, q1, p1, b0, b1);
+            }
           }
-        }
-        const unsigned char* vs = st + 16 * F::K_PITCH + 2 * t4 * F::V_PITCH + gr * 4;
 #pragma unroll
-        for (int j = 0; j < D / 8; ++j) {
-          float c[4] = {0.f, 0.f, 0.f, 0.f};
+          for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) x[nt][e] = (c[0][nt][e] + c[1][nt][e]) + (c[0][nt][2 + e] + c[1][nt][2 + e]);
+        }
+        // An infinite key gives 0 * inf among the parts' products: such a score is taken again from whole operands.
+        if (__any_sync(0xffffffffu, !(x[0][0] == x[0][0] && x[0][1] == x[0][1] && x[1][0] == x[1][0] && x[1][1] == x[1][1]))) {
+#pragma unroll
+          for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+              if (x[nt][e] != x[nt][e] && gr < (int)rows) {
+                const unsigned char* k = st + (nt * 8 + 2 * t4 + e) * F::K_PITCH;
+                float t = 0.f;
+                for (int i = 0; i < D; ++i)
+                  t = fmaf(load_float(g.q.p, (uint64_t)here.s * g.q.ld + (uint64_t)(head0 + gr) * D + i, g.q.bf16), load_float(k, i, F::BF), t);
+                x[nt][e] = t;
+              }
+        }
+
+        // running softmax: new maximum, the factor of what was summed before, the weights
+#pragma unroll
+        for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) x[nt][e] = (live >> (nt * 8 + 2 * t4 + e)) & 1 ? x[nt][e] * a.scale_log2 : -INFINITY;
+        float top = fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[1][0], x[1][1]));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        top = fmaxf(top, m);
+        const float f = exp2_fast(m - top);
+        m = top;
+#pragma unroll
+        for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) x[nt][e] = exp2_fast(x[nt][e] - m);
+        l = fmaf(l, f, (x[0][0] + x[0][1]) + (x[1][0] + x[1][1]));
+
+        // rows = rows * factor + weights x values
+        if constexpr (F::BF) {
+          uint32_t w[3][2];
 #pragma unroll
           for (int nt = 0; nt < 2; ++nt) {
-            const float u = *reinterpret_cast<const float*>(vs + nt * 8 * F::V_PITCH + j * 32);
-            const float v = *reinterpret_cast<const float*>(vs + (nt * 8 + 1) * F::V_PITCH + j * 32);
-            const uint32_t b0 = tf32_of(u), b1 = tf32_of(v);
-            mma_tf32(c, lo[nt], b0, b1);
-            mma_tf32(c, hi[nt], __float_as_uint(u - __uint_as_float(b0)), __float_as_uint(v - __uint_as_float(b1)));
-            mma_tf32(c, hi[nt], b0, b1);
+            float u = x[nt][0], v = x[nt][1];
+            w[0][nt] = bf16x2(u, v);
+            u -= low_of(w[0][nt]); v -= high_of(w[0][nt]);
+            w[1][nt] = bf16x2(u, v);
+            if constexpr (EXACT) w[2][nt] = bf16x2(u - low_of(w[1][nt]), v - high_of(w[1][nt]));
           }
-          float* r = o[j];
-          r[0] = fmaf(r[0], f0, c[0]); r[1] = fmaf(r[1], f0, c[1]);
-          r[2] = fmaf(r[2], f1, c[2]); r[3] = fmaf(r[3], f1, c[3]);
-        }
-      }
-    }
-
-    // ---- the warps' (maximum, sum, rows) into one, SLAB columns at a time
-    l0 += __shfl_xor_sync(0xffffffffu, l0, 1); l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
-    l1 += __shfl_xor_sync(0xffffffffu, l1, 1); l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
-    if (t4 == 0) {
-      ml[(warp * 16 + gr) * 2] = m0; ml[(warp * 16 + gr) * 2 + 1] = l0;
-      ml[(warp * 16 + gr + 8) * 2] = m1; ml[(warp * 16 + gr + 8) * 2 + 1] = l1;
-    }
-    __syncthreads();
-    {
-      float t0 = -FLT_MAX, t1 = -FLT_MAX;
-      for (int w = 0; w < F::WARPS; ++w) { t0 = fmaxf(t0, ml[(w * 16 + gr) * 2]); t1 = fmaxf(t1, ml[(w * 16 + gr + 8) * 2]); }
-      m0 = exp2_fast(m0 - t0); m1 = exp2_fast(m1 - t1);                        // this warp's factors from here on
-    }
-    float* part = a.part + ((uint64_t)block * 2 + (piece_i ? 1 : 0)) * 16 * (D + 2);
+          if constexpr (!EXACT)
+            if (__any_sync(0xffffffffu, f != 1.f)) {
 #pragma unroll
-    for (int at = 0; at < D; at += F::SLAB) {
-      if (at) __syncthreads();
+              for (int j = 0; j < D / 8; ++j)
 #pragma unroll
-      for (int j = 0; j < F::SLAB / 8; ++j) {
-        const float* r = o[at / 8 + j];
-        float* to = slab + (warp * 16 + gr) * F::SLAB_PITCH + j * 8 + 2 * t4;
-        *reinterpret_cast<float2*>(to) = make_float2(r[0] * m0, r[1] * m0);
-        *reinterpret_cast<float2*>(to + 8 * F::SLAB_PITCH) = make_float2(r[2] * m1, r[3] * m1);
-      }
-      __syncthreads();
-      for (int i = tid; i < (int)rows * F::SLAB; i += F::THREADS) {
-        const int r = i / F::SLAB, c = i % F::SLAB;
-        float v = 0.f;
-        for (int w = 0; w < F::WARPS; ++w) v += slab[(w * 16 + r) * F::SLAB_PITCH + c];
-        if (whole) {
-          float top = -FLT_MAX, den = 0.f;
-          for (int w = 0; w < F::WARPS; ++w) top = fmaxf(top, ml[(w * 16 + r) * 2]);
-          for (int w = 0; w < F::WARPS; ++w) den += ml[(w * 16 + r) * 2 + 1] * exp2_fast(ml[(w * 16 + r) * 2] - top);
-          store_float(g.out, (uint64_t)here.s * out_cols + (uint64_t)(head0 + r) * D + at + c, g.out_bf16, v / (den < FLT_MIN ? FLT_MIN : den));
+                for (int e = 0; e < ROW_REGS; ++e) o[j][e] *= f;
+            }
+          const uint32_t vb = v_at + ((lane & 7) + ((lane >> 3) & 1) * 8) * F::V_PITCH + (lane >> 4) * 16;
+#pragma unroll
+          for (int j = 0; j < D / 16; ++j) {
+            uint32_t b[4];
+            ldmatrix4_t(b, vb + j * 32);
+#pragma unroll
+            for (int hf = 0; hf < 2; ++hf) {
+              float* r = o[2 * j + hf];
+              if constexpr (EXACT) {
+                float c[4] = {0.f, 0.f, 0.f, 0.f};
+                mma_bf16(c, 0u, w[2][0], 0u, w[2][1], b[2 * hf], b[2 * hf + 1]);
+                mma_bf16(c, w[0][0], w[1][0], w[0][1], w[1][1], b[2 * hf], b[2 * hf + 1]);
+                r[0] = fmaf(r[0], f, c[0] + c[2]);
+                r[1] = fmaf(r[1], f, c[1] + c[3]);
+              } else {
+                mma_bf16(r, w[0][0], w[1][0], w[0][1], w[1][1], b[2 * hf], b[2 * hf + 1]);
+              }
+            }
+          }
         } else {
-          part[r * D + at + c] = v;
+          uint32_t hi[2][2], lo[2][2];
+#pragma unroll
+          for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              hi[nt][e] = tf32_of(x[nt][e]);
+              lo[nt][e] = __float_as_uint(x[nt][e] - __uint_as_float(hi[nt][e]));
+            }
+          const uint32_t vs = v_at + 2 * t4 * F::V_PITCH + gr * 4;
+#pragma unroll
+          for (int j = 0; j < D / 8; ++j) {
+            float c[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int nt = 0; nt < 2; ++nt) {
+              const float u = lds1(vs + nt * 8 * F::V_PITCH + j * 32);
+              const float v = lds1(vs + (nt * 8 + 1) * F::V_PITCH + j * 32);
+              const uint32_t b0 = tf32_of(u), b1 = tf32_of(v);
+              mma_tf32(c, hi[nt][0], 0u, hi[nt][1], 0u, __float_as_uint(u - __uint_as_float(b0)), __float_as_uint(v - __uint_as_float(b1)));
+              mma_tf32(c, hi[nt][0], lo[nt][0], hi[nt][1], lo[nt][1], b0, b1);
+            }
+            o[j][0] = fmaf(o[j][0], f, c[0] + c[2]);
+            o[j][1] = fmaf(o[j][1], f, c[1] + c[3]);
+          }
         }
       }
+
+      // ---- the sequence's result, or its part of one
+      l += __shfl_xor_sync(0xffffffffu, l, 1);
+      l += __shfl_xor_sync(0xffffffffu, l, 2);
+      if (gr < (int)rows) {
+        if (whole) {
+          const float den = l < FLT_MIN ? FLT_MIN : l;
+          const uint64_t at = (uint64_t)here.s * out_cols + (uint64_t)(head0 + gr) * D + 2 * t4;
+#pragma unroll
+          for (int j = 0; j < D / 8; ++j) {
+            float u = o[j][0], v = o[j][1];
+            if constexpr (ROW_REGS == 4) { u += o[j][2]; v += o[j][3]; }
+            u /= den; v /= den;
+            if (g.out_bf16)
+              *reinterpret_cast<uint32_t*>(reinterpret_cast<uint16_t*>(g.out) + at + j * 8) =
+                  (uint32_t)f32_to_bf16_bits(__float_as_uint(u)) | ((uint32_t)f32_to_bf16_bits(__float_as_uint(v)) << 16);
+            else *reinterpret_cast<float2*>(reinterpret_cast<float*>(g.out) + at + j * 8) = make_float2(u, v);
+          }
+        } else {
+          float* part = a.part + ((uint64_t)task * 2 + (piece ? 1 : 0)) * a.slot;
+#pragma unroll
+          for (int j = 0; j < D / 8; ++j) {
+            float u = o[j][0], v = o[j][1];
+            if constexpr (ROW_REGS == 4) { u += o[j][2]; v += o[j][3]; }
+            *reinterpret_cast<float2*>(part + gr * D + j * 8 + 2 * t4) = make_float2(u, v);
+          }
+          if (t4 == 0) *reinterpret_cast<float2*>(part + a.slot / (D + 4) * D + gr * 4) = make_float2(m, l);
+        }
+      }
+      left -= steps;
+      here.tile += steps;
+      if (here.tile == here.tiles) next_sequence(here);
     }
-    if (!whole && tid < 16) {
-      float top = -FLT_MAX, den = 0.f;
-      for (int w = 0; w < F::WARPS; ++w) top = fmaxf(top, ml[(w * 16 + tid) * 2]);
-      for (int w = 0; w < F::WARPS; ++w) den += ml[(w * 16 + tid) * 2 + 1] * exp2_fast(ml[(w * 16 + tid) * 2] - top);
-      part[16 * D + tid * 2] = top;
-      part[16 * D + tid * 2 + 1] = den;
-    }
-    left -= steps;
-    here.tile += steps;
-    if (here.tile == here.tiles) next_job(here);
+    cp_async_wait(0);
+    __syncwarp();
   }
-  cp_async_wait(0);
 }
 
-// Joins a (sequence, head) whose tiles lie in several blocks' runs: block (c, r) is query row r of the piece that ends block
-// c's run, if c is the first of its blocks.  rows = sum over the blocks, in their order, of rows_c 2^(m_c - m) / sum l_c 2^(m_c - m).
+// Joins the sequences whose tiles lie in several runs: block (i, h) is query head h of sequence i, or, with fewer runs than
+// sequences, of the sequence that run i ends in, if that run is its first.
+// rows = sum over the runs, in their order, of rows_c 2^(m_c - m) / sum l_c 2^(m_c - m).
 template <int D>
-__global__ void __launch_bounds__(256) attention_pages_join_kernel(const __grid_constant__ AttnPlan a, uint32_t blocks) {
-  constexpr int LANES = D / 4, TEAMS = 256 / LANES;          // a team a block's row, a float4 a lane
-  __shared__ __align__(16) float sums[TEAMS][D];
-  __shared__ float red[256 / 32], dens[TEAMS];
+__global__ void __launch_bounds__(512) attention_pages_join_kernel(const __grid_constant__ AttnPlan a) {
+  constexpr int LANES = D / 4;           // a team a run's row, a float4 a lane
+  extern __shared__ __align__(16) float sums[];              // [teams][D]
+  __shared__ float red[16], dens[512 / LANES];
   pdl_enter();
   const AttnPagesArgs& g = a.g;
-  const int tid = threadIdx.x;
-  const uint32_t c0 = blockIdx.x, r = blockIdx.y, n = (uint32_t)g.n;
-  const uint32_t total = a.prefix[n];
-  const uint32_t next = run_start(total, c0 + 1, blocks), mine = run_start(total, c0, blocks);
-  if (mine >= next || next >= total) return;                 // an empty run, or nothing goes on behind it
-  uint32_t s = 0, hi = n - 1;
-  while (s < hi) {
-    const uint32_t mid = (s + hi + 1) / 2;
-    if (a.prefix[mid] <= next) s = mid; else hi = mid - 1;
+  const int tid = threadIdx.x, threads = blockDim.x, teams = threads / LANES;
+  const uint32_t n = (uint32_t)g.n, total = a.prefix[n], head = blockIdx.y;
+  if (total == 0) return;
+  uint32_t s = blockIdx.x;
+  if (a.runs < n) {
+    const uint32_t mine = run_start(total, blockIdx.x, a.runs), next = run_start(total, blockIdx.x + 1, a.runs);
+    if (mine >= next || next >= total) return;               // an empty run, or nothing goes on behind it
+    s = sequence_of(a.prefix, n, next);
+    if (a.prefix[s] < mine || a.prefix[s] == next) return;   // it began before this run, or begins behind it
   }
-  const uint32_t tiles = (a.prefix[s + 1] - a.prefix[s]) / a.jobs, job = (next - a.prefix[s]) / tiles;
-  const uint32_t first = a.prefix[s] + job * tiles, last = first + tiles - 1;
-  if (first == next || first < mine) return;                 // the piece starts behind the run, or before it: another block's
-  const uint32_t kvh = job / a.row_tiles, r0 = job % a.row_tiles * 16;
-  if (r >= a.group - r0) return;
-  const uint32_t c1 = run_owner(total, last, blocks);
-  const auto piece = [&](uint32_t c) { return a.part + ((uint64_t)c * 2 + (c == c0 && first != mine ? 1 : 0)) * 16 * (D + 2); };
-  // an empty run lies between two others only where there are fewer tiles than blocks: it holds nothing of the piece
-  const auto there = [&](uint32_t c) { return run_start(total, c, blocks) < run_start(total, c + 1, blocks); };
+  const uint32_t first = a.prefix[s], end = a.prefix[s + 1];
+  if (first >= end) return;
+  const uint32_t c0 = run_owner(total, first, a.runs), c1 = run_owner(total, end - 1, a.runs);
+  if (c0 == c1) return;                                      // written whole
+  const uint32_t in = head % a.group, job = head / a.group * a.row_tiles + in / HEADS, r = in % HEADS;
+  const uint32_t ml = a.slot / (D + 4) * D + r * 4;
+  const bool later = run_start(total, c0, a.runs) != first;  // the sequence is not the first of its first run
+  const auto piece = [&](uint32_t c) { return a.part + (((uint64_t)c * a.jobs + job) * 2 + (c == c0 && later ? 1 : 0)) * a.slot; };
+  // an empty run lies between two others only where there are fewer tiles than runs: it holds nothing
+  const auto there = [&](uint32_t c) { return run_start(total, c, a.runs) < run_start(total, c + 1, a.runs); };
   float top = -FLT_MAX;
-  for (uint32_t c = c0 + tid; c <= c1; c += 256)
-    if (there(c)) top = fmaxf(top, piece(c)[16 * D + r * 2]);
+  for (uint32_t c = c0 + tid; c <= c1; c += threads)
+    if (there(c)) top = fmaxf(top, piece(c)[ml]);
 #pragma unroll
   for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
   if ((tid & 31) == 0) red[tid >> 5] = top;
   __syncthreads();
-  for (int w = 0; w < 8; ++w) top = fmaxf(top, red[w]);
+  for (int w = 0; w < threads / 32; ++w) top = fmaxf(top, red[w]);
   const int team = tid / LANES, lane = tid % LANES;
-  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-  float den = 0.f;
-  if (team < TEAMS)
-    for (uint32_t c = c0 + team; c <= c1; c += TEAMS)
+  if (team < teams) {
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    float den = 0.f;
+#pragma unroll 4
+    for (uint32_t c = c0 + team; c <= c1; c += teams)
       if (there(c)) {
         const float* p = piece(c);
-        const float f = exp2_fast(p[16 * D + r * 2] - top);
+        const float f = exp2_fast(p[ml] - top);
         const float4 x = *reinterpret_cast<const float4*>(p + r * D + lane * 4);
-        den = fmaf(p[16 * D + r * 2 + 1], f, den);
+        den = fmaf(p[ml + 1], f, den);
         v.x = fmaf(x.x, f, v.x); v.y = fmaf(x.y, f, v.y); v.z = fmaf(x.z, f, v.z); v.w = fmaf(x.w, f, v.w);
       }
-  if (team < TEAMS) {
-    *reinterpret_cast<float4*>(&sums[team][lane * 4]) = v;
+    *reinterpret_cast<float4*>(sums + team * D + lane * 4) = v;
     if (lane == 0) dens[team] = den;
   }
   __syncthreads();
-  if (tid < D) {
+  for (int j = tid; j < D; j += threads) {
     float t = 0.f, l = 0.f;
-    for (int w = 0; w < TEAMS; ++w) { t += sums[w][tid]; l += dens[w]; }
-    const uint32_t head = kvh * a.group + r0 + r;
-    store_float(g.out, (uint64_t)s * a.g.cache.heads * D + (uint64_t)head * D + tid, g.out_bf16, t / (l < FLT_MIN ? FLT_MIN : l));
+    for (int w = 0; w < teams; ++w) { t += sums[w * D + j]; l += dens[w]; }
+    store_float(g.out, (uint64_t)s * g.cache.heads * D + (uint64_t)head * D + j, g.out_bf16, t / (l < FLT_MIN ? FLT_MIN : l));
   }
 }
-
-// The tiles a sequence can have at most, from the shapes alone.
-uint64_t attention_tiles(const AttnPagesArgs& g, int tile) {
-  uint64_t p = (uint64_t)g.cache.width * g.cache.page;
-  if (g.window && p > g.window) p = g.window;
-  return (p + tile - 1) / tile;
-}
-struct AttnScratch { float* part; uint32_t* prefix; };
 
 // The current device's SMs, asked for once a device.
 int sm_count() {
@@ -632,80 +595,120 @@ int sm_count() {
   return v;
 }
 
+// How a launch of `n` sequences is cut, from the shapes alone.
+struct Cut { uint64_t n; uint32_t group, row_tiles, jobs, runs, slot, workers; uint64_t tiles; };
+Cut cut_of(const AttnPagesArgs& g, uint64_t left, int dim, int workers) {
+  Cut c;
+  c.group = g.cache.heads / g.cache.kv_heads;
+  c.row_tiles = (c.group + HEADS - 1) / HEADS;
+  c.jobs = g.cache.kv_heads * c.row_tiles;
+  c.slot = (c.group < HEADS ? c.group : HEADS) * (dim + 4);
+  c.workers = workers;
+  uint64_t positions = (uint64_t)g.cache.width * g.cache.page;
+  if (g.window && positions > g.window) positions = g.window;
+  c.tiles = (positions + 15) / 16;                           // a sequence's, at most (below 2^28)
+  c.n = left < MAX_SEQUENCES ? left : MAX_SEQUENCES;
+  if (c.tiles && c.n > 0xffffffffull / c.tiles) c.n = 0xffffffffull / c.tiles;
+  // Runs: as many as give every warp one (run, head).  With so many heads that a warp more or less in that division weighs,
+  // the count whose last round of warps is fullest.
+  uint32_t runs = c.jobs < c.workers ? c.workers / c.jobs : 1;
+  if (runs < 8) {
+    const auto rounds = [&](uint32_t r) { return (double)(((uint64_t)r * c.jobs + c.workers - 1) / c.workers) / r; };
+    for (uint32_t r = runs + 1; r <= 16; ++r)
+      if (rounds(r) < 0.95 * rounds(runs)) runs = r;
+  }
+  if (runs > c.n * c.tiles) runs = (uint32_t)(c.n * c.tiles);
+  c.runs = runs < 1 ? 1 : runs;
+  return c;
+}
+
 template <typename KV, int D, int QP, bool EXACT>
-cudaError_t attention_form(const AttnPagesArgs& g, int sms, const AttnScratch& scratch, int* launches, cudaStream_t stream) {
+cudaError_t attention_form(const AttnPagesArgs& g, void* scratch, int* launches, cudaStream_t stream) {
   using F = Form<KV, D>;
+  const int workers = F::BLOCKS * F::WARPS * sm_count();
   AttnPlan a;
   a.g = g;
   a.page_shift = 31 - __builtin_clz(g.cache.page);
   a.page_magic = (1ull << (32 + a.page_shift)) / g.cache.page + 1;
-  a.group = g.cache.heads / g.cache.kv_heads;
-  a.row_tiles = (a.group + 15) / 16;
-  a.jobs = g.cache.kv_heads * a.row_tiles;
   a.scale_log2 = g.scale * 1.44269504088896340736f;
-  a.part = scratch.part; a.prefix = scratch.prefix;
   const int limit = 228 * 1024 / F::BLOCKS - 1024 - 256;   // a block's share of an SM's shared memory, less what the launch and the statics take
-  const uint64_t per_sequence = attention_tiles(g, F::TILE) * a.jobs;
-  if (per_sequence > 0xffffffffull) return cudaErrorNotSupported;
   cudaError_t e = ensure_dynamic_smem((const void*)attention_pages_kernel<KV, D, QP, EXACT>, limit);
   if (e != cudaSuccess) return e;
   for (uint64_t at = 0; at < g.n;) {
-    uint64_t rows = g.n - at < MAX_SEQUENCES ? g.n - at : MAX_SEQUENCES;
-    if (per_sequence && rows > 0xffffffffull / per_sequence) rows = 0xffffffffull / per_sequence;
-    a.g.n = rows;
+    const Cut c = cut_of(g, g.n - at, D, workers);
+    a.group = c.group; a.row_tiles = c.row_tiles; a.jobs = c.jobs; a.runs = c.runs; a.slot = c.slot;
+    a.prefix = (uint32_t*)scratch;
+    a.part = (float*)((char*)scratch + 4096);
+    a.g.n = c.n;
     a.g.cache.table = g.cache.table + at * g.cache.width;
     a.g.positions = g.positions + at;
     a.g.q.p = (const char*)g.q.p + at * g.q.ld * (g.q.bf16 ? 2 : 4);
     a.g.out = (char*)g.out + at * g.cache.heads * D * (g.out_bf16 ? 2 : 4);
-    const int fixed = F::prefix_bytes((uint32_t)rows) + F::ML + F::q_bytes(QP);
+    const int fixed = F::prefix_bytes((uint32_t)c.n);
     a.stages = (limit - fixed) / (F::WARPS * F::STAGE);
     if (a.stages > MAX_STAGES) a.stages = MAX_STAGES;
     if (a.stages < 2) return cudaErrorNotSupported;
-    uint64_t blocks = (uint64_t)F::BLOCKS * sms;
-    if (blocks > rows * per_sequence) blocks = rows * per_sequence;   // no more than the tiles there can be
-    if (blocks < 1) blocks = 1;
+    uint64_t blocks = ((uint64_t)c.runs * c.jobs + F::WARPS - 1) / F::WARPS;
+    if (blocks > (uint64_t)F::BLOCKS * sm_count()) blocks = (uint64_t)F::BLOCKS * sm_count();
     launch_pdl(attention_pages_kernel<KV, D, QP, EXACT>, dim3((unsigned)blocks), dim3(F::THREADS), fixed + a.stages * F::WARPS * F::STAGE, stream, a);
     e = cudaGetLastError();
     if (e != cudaSuccess) return e;
     ++*launches;
-    if (blocks > 1 && per_sequence > a.jobs) {               // a (sequence, head) of one tile is never divided
-      launch_pdl(attention_pages_join_kernel<D>, dim3((unsigned)blocks, a.group < 16 ? a.group : 16), dim3(256), 0, stream, a, (uint32_t)blocks);
+    if (c.runs > 1 && c.tiles > 1) {                         // a sequence of one tile is never divided
+      // a sequence's runs over as many teams as leave each a few
+      constexpr int LANES = D / 4;
+      const uint64_t each = c.runs / c.n;
+      int threads = (int)(each > 64 ? 512 : (each > 8 ? 256 : (each > 2 ? 128 : 64)));
+      if (threads < LANES) threads = LANES;
+      launch_pdl(attention_pages_join_kernel<D>, dim3((unsigned)(c.n < c.runs ? c.n : c.runs), g.cache.heads), dim3(threads),
+                 threads / LANES * D * sizeof(float), stream, a);
       e = cudaGetLastError();
       if (e != cudaSuccess) return e;
       ++*launches;
     }
-    at += rows;
+    at += c.n;
   }
   return cudaSuccess;
 }
 
 // The form for the types: an operand's parts as the precision note says.
 template <int D>
-cudaError_t attention_dim(const AttnPagesArgs& g, int sms, const AttnScratch& s, int* launches, cudaStream_t stream) {
-  if (!g.cache.bf16) return attention_form<float, D, 2, true>(g, sms, s, launches, stream);
-  if (g.q.bf16) return g.out_bf16 ? attention_form<uint16_t, D, 1, false>(g, sms, s, launches, stream)
-                                  : attention_form<uint16_t, D, 1, true>(g, sms, s, launches, stream);
-  return g.out_bf16 ? attention_form<uint16_t, D, 2, false>(g, sms, s, launches, stream)
-                    : attention_form<uint16_t, D, 3, true>(g, sms, s, launches, stream);
+cudaError_t attention_dim(const AttnPagesArgs& g, void* scratch, int* launches, cudaStream_t stream) {
+  if (!g.cache.bf16) return attention_form<float, D, 2, true>(g, scratch, launches, stream);
+  if (g.q.bf16) return g.out_bf16 ? attention_form<uint16_t, D, 1, false>(g, scratch, launches, stream)
+                                  : attention_form<uint16_t, D, 1, true>(g, scratch, launches, stream);
+  return g.out_bf16 ? attention_form<uint16_t, D, 2, false>(g, scratch, launches, stream)
+                    : attention_form<uint16_t, D, 3, true>(g, scratch, launches, stream);
+}
+
+template <int D>
+int workers_of(int bf16) {
+  return (bf16 ? Form<uint16_t, D>::BLOCKS * Form<uint16_t, D>::WARPS : Form<float, D>::BLOCKS * Form<float, D>::WARPS) * sm_count();
 }
 
 }  // namespace
 
 bool attention_pages_dim_ok(uint32_t d) { return d == 32 || d == 64 || d == 96 || d == 128 || d == 192 || d == 256; }
 
-// Two pieces for every block that may be launched (at most four an SM), and the prefix sums.
-size_t attention_pages_scratch_bytes(uint32_t dim) {
-  return (size_t)4 * sm_count() * 2 * 16 * (dim + 2) * sizeof(float) + (MAX_SEQUENCES + 1) * sizeof(uint32_t);
+// The prefix sums, and two pieces for every (run, head) of the largest launch.
+size_t attention_pages_scratch_bytes(const AttnPagesArgs& g) {
+  int workers = 0;
+  switch (g.cache.dim) {
+    case 32: workers = workers_of<32>(g.cache.bf16); break;
+    case 64: workers = workers_of<64>(g.cache.bf16); break;
+    case 96: workers = workers_of<96>(g.cache.bf16); break;
+    case 128: workers = workers_of<128>(g.cache.bf16); break;
+    case 192: workers = workers_of<192>(g.cache.bf16); break;
+    default: workers = workers_of<256>(g.cache.bf16); break;
+  }
+  const Cut c = cut_of(g, g.n, (int)g.cache.dim, workers);
+  return 4096 + (size_t)c.runs * c.jobs * 2 * c.slot * sizeof(float);
 }
 
 cudaError_t launch_attention_pages(const AttnPagesArgs& g, void* scratch, int* launches, cudaStream_t stream) {
   *launches = 0;
   if (g.n == 0) return cudaSuccess;
-  const int sms = sm_count();
-  AttnScratch s;
-  s.part = (float*)scratch;
-  s.prefix = (uint32_t*)(s.part + (size_t)4 * sms * 2 * 16 * (g.cache.dim + 2));
-#define GO(D) case D: return attention_dim<D>(g, sms, s, launches, stream)
+#define GO(D) case D: return attention_dim<D>(g, scratch, launches, stream)
   switch (g.cache.dim) {
     GO(32); GO(64); GO(96); GO(128); GO(192); GO(256);
     default: return cudaErrorNotSupported;

@@ -280,7 +280,7 @@ struct AttnPagesArgs {
   int* err = nullptr;
 };
 bool attention_pages_dim_ok(uint32_t dim);
-size_t attention_pages_scratch_bytes(uint32_t dim);   // of the current device
+size_t attention_pages_scratch_bytes(const AttnPagesArgs& args);   // on the current device
 cudaError_t launch_attention_pages(const AttnPagesArgs& args, void* scratch, int* launches, cudaStream_t stream);
 
 // ---- token log probabilities (k_logprob.cu) -------------------------------------

@@ -16,7 +16,7 @@ cudaError_t launch_rope_append_pages(const AppendArgs& g, cudaStream_t) {
   return launched();
 }
 bool attention_pages_dim_ok(uint32_t d) { return d == 32 || d == 64 || d == 96 || d == 128 || d == 192 || d == 256; }
-size_t attention_pages_scratch_bytes(uint32_t dim) { return (size_t)dim * 64 + 256; }
+size_t attention_pages_scratch_bytes(const AttnPagesArgs& g) { return g.n * 64 + 256; }
 cudaError_t launch_attention_pages(const AttnPagesArgs&, void*, int* launches, cudaStream_t) { *launches = 2; return launched(); }
 cudaError_t launch_token_logprobs(const LogprobArgs&, cudaStream_t) { return launched(); }
 cudaError_t launch_token_logprobs_backward(const LogprobGradArgs&, cudaStream_t) { return launched(); }
