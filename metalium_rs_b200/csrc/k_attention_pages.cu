@@ -10,9 +10,10 @@
 // not, which a second kernel joins.  The lengths are on the device, so the list is made there, from a prefix sum.  After that
 // sum no warp waits for another.
 //
-// A warp's pipeline: it copies its 16 keys and 16 values of a tile to its own shared memory by 16-byte asynchronous copies, a
-// few tiles ahead (row addresses through the page table, fetched one tile before they are used), and keeps its own running
-// maximum, sum and rows.
+// A warp's pipeline: it copies its 16 keys and 16 values of a tile to its own shared memory by 16-byte asynchronous copies, as
+// many tiles ahead as it has room for (the place of a tile's keys is filled again as soon as its scores are taken, that of its
+// values after the product with them; row addresses through the page table, fetched one tile before they are used), and keeps
+// its own running maximum, sum and rows.
 //
 // Precision: keys and values are the cache's own values.  The tensor cores' tile has sixteen rows, and a head takes two of
 // them: row r has an operand's leading part and row r + 8 the next one, so one product does both.  On the BF16 path an F32
@@ -78,8 +79,9 @@ __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commi
 // all but the latest `pending` groups of this thread have arrived
 __device__ __forceinline__ void cp_async_wait(int pending) {
   if (pending <= 0) asm volatile("cp.async.wait_group 0;" ::: "memory");
-  else if (pending == 1) asm volatile("cp.async.wait_group 1;" ::: "memory");
-  else asm volatile("cp.async.wait_group 2;" ::: "memory");
+  else if (pending <= 3) asm volatile("cp.async.wait_group 3;" ::: "memory");
+  else if (pending <= 5) asm volatile("cp.async.wait_group 5;" ::: "memory");
+  else asm volatile("cp.async.wait_group 7;" ::: "memory");
 }
 __device__ __forceinline__ void ldmatrix4(uint32_t* r, uint32_t at) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
@@ -265,23 +267,28 @@ __global__ void __launch_bounds__(Form<KV, D>::THREADS, Form<KV, D>::BLOCKS) att
     const uint64_t head_at = (uint64_t)kvh * D * sizeof(KV) + (lane % F::LANES) * 16;
     const char *key_at = (const char*)cache.keys + head_at, *value_at = (const char*)cache.values + head_at;
     int issue_stage = 0;
-    const auto issue = [&]() {
+    const auto copy = [&](uint32_t at, const char* from_at, int pitch) {
+#pragma unroll
+      for (int i = 0; i < F::REST; ++i) {
+        const int r = i * F::ROWS + lane / F::LANES;
+        const int32_t from = __shfl_sync(0xffffffffu, row, r);
+        const bool on = from >= 0;
+        const char* x = from_at + (uint64_t)(uint32_t)(on ? from : 0) * ld;
+#pragma unroll
+        for (int c = 0; c < F::PIECES; ++c) cp_async16(at + r * pitch + c * F::LANES * 16, x + c * F::LANES * 16, on);
+      }
+    };
+    const auto issue_keys = [&]() {      // a group of copies each, the keys' and the values' of a tile in turn
       if (to_issue) {
         const uint32_t there = __ballot_sync(0xffffffffu, row >= 0);
         if (lane == 0) valid[warp][issue_stage] = there & 0xffffu;
-        const uint32_t at = to + issue_stage * F::STAGE;
-#pragma unroll
-        for (int i = 0; i < F::REST; ++i) {
-          const int r = i * F::ROWS + lane / F::LANES;
-          const int32_t from = __shfl_sync(0xffffffffu, row, r);
-          const bool on = from >= 0;
-          const uint64_t off = (uint64_t)(uint32_t)(on ? from : 0) * ld;
-#pragma unroll
-          for (int c = 0; c < F::PIECES; ++c) {
-            cp_async16(at + r * F::K_PITCH + c * F::LANES * 16, key_at + off + c * F::LANES * 16, on);
-            cp_async16(at + 16 * F::K_PITCH + r * F::V_PITCH + c * F::LANES * 16, value_at + off + c * F::LANES * 16, on);
-          }
-        }
+        copy(to + issue_stage * F::STAGE, key_at, F::K_PITCH);
+      }
+      cp_async_commit();
+    };
+    const auto issue_values = [&]() {
+      if (to_issue) {
+        copy(to + issue_stage * F::STAGE + 16 * F::K_PITCH, value_at, F::V_PITCH);
         --to_issue;
         if (++ahead.tile == ahead.tiles) next_sequence(ahead);
         look_up();
@@ -289,7 +296,7 @@ __global__ void __launch_bounds__(Form<KV, D>::THREADS, Form<KV, D>::BLOCKS) att
       cp_async_commit();
       if (++issue_stage == a.stages) issue_stage = 0;
     };
-    for (int i = 0; i + 1 < a.stages; ++i) issue();
+    for (int i = 0; i < a.stages; ++i) { issue_keys(); issue_values(); }
 
     // ---- the run's sequences, one after another
     Cursor here;
@@ -335,9 +342,8 @@ __global__ void __launch_bounds__(Form<KV, D>::THREADS, Form<KV, D>::BLOCKS) att
         for (int e = 0; e < ROW_REGS; ++e) o[j][e] = 0.f;
       float m = -FLT_MAX, l = 0.f;       // row gr's; the sum is this lane's own
       for (uint32_t step = 0; step < steps; ++step) {
-        cp_async_wait(a.stages - 2);
-        __syncwarp();                    // every lane's copies of this stage are in, and every lane is done with the stage before
-        issue();
+        cp_async_wait(2 * a.stages - 1);
+        __syncwarp();                    // every lane's copies of the keys are in
         const unsigned char* st = stages + stage * F::STAGE;
         const uint32_t live = valid[warp][stage];
         if (++stage == a.stages) stage = 0;
@@ -404,6 +410,9 @@ __global__ void __launch_bounds__(Form<KV, D>::THREADS, Form<KV, D>::BLOCKS) att
               }
         }
 
+        __syncwarp();                    // every lane is done with the keys
+        issue_keys();
+
         // running softmax: new maximum, the factor of what was summed before, the weights
 #pragma unroll
         for (int nt = 0; nt < 2; ++nt)
@@ -422,6 +431,8 @@ __global__ void __launch_bounds__(Form<KV, D>::THREADS, Form<KV, D>::BLOCKS) att
         l = fmaf(l, f, (x[0][0] + x[0][1]) + (x[1][0] + x[1][1]));
 
         // rows = rows * factor + weights x values
+        cp_async_wait(2 * a.stages - 1);
+        __syncwarp();                    // every lane's copies of the values are in
         if constexpr (F::BF) {
           uint32_t w[3][2];
 #pragma unroll
@@ -483,6 +494,8 @@ __global__ void __launch_bounds__(Form<KV, D>::THREADS, Form<KV, D>::BLOCKS) att
             o[j][1] = fmaf(o[j][1], f, c[1] + c[3]);
           }
         }
+        __syncwarp();                    // every lane is done with the values
+        issue_values();
       }
 
       // ---- the sequence's result, or its part of one
@@ -526,15 +539,14 @@ __global__ void __launch_bounds__(Form<KV, D>::THREADS, Form<KV, D>::BLOCKS) att
 // sequences, of the sequence that run i ends in, if that run is its first.
 // rows = sum over the runs, in their order, of rows_c 2^(m_c - m) / sum l_c 2^(m_c - m).
 template <int D>
-__global__ void __launch_bounds__(512) attention_pages_join_kernel(const __grid_constant__ AttnPlan a) {
+__global__ void __launch_bounds__(1024) attention_pages_join_kernel(const __grid_constant__ AttnPlan a) {
   constexpr int LANES = D / 4;           // a team a run's row, a float4 a lane
   extern __shared__ __align__(16) float sums[];              // [teams][D]
-  __shared__ float red[16], dens[512 / LANES];
+  __shared__ float tops[1024 / LANES], dens[1024 / LANES];
   pdl_enter();
   const AttnPagesArgs& g = a.g;
   const int tid = threadIdx.x, threads = blockDim.x, teams = threads / LANES;
   const uint32_t n = (uint32_t)g.n, total = a.prefix[n], head = blockIdx.y;
-  if (total == 0) return;
   uint32_t s = blockIdx.x;
   if (a.runs < n) {
     const uint32_t mine = run_start(total, blockIdx.x, a.runs), next = run_start(total, blockIdx.x + 1, a.runs);
@@ -552,34 +564,48 @@ __global__ void __launch_bounds__(512) attention_pages_join_kernel(const __grid_
   const auto piece = [&](uint32_t c) { return a.part + (((uint64_t)c * a.jobs + job) * 2 + (c == c0 && later ? 1 : 0)) * a.slot; };
   // an empty run lies between two others only where there are fewer tiles than runs: it holds nothing
   const auto there = [&](uint32_t c) { return run_start(total, c, a.runs) < run_start(total, c + 1, a.runs); };
-  float top = -FLT_MAX;
-  for (uint32_t c = c0 + tid; c <= c1; c += threads)
-    if (there(c)) top = fmaxf(top, piece(c)[ml]);
-#pragma unroll
-  for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  if ((tid & 31) == 0) red[tid >> 5] = top;
-  __syncthreads();
-  for (int w = 0; w < threads / 32; ++w) top = fmaxf(top, red[w]);
   const int team = tid / LANES, lane = tid % LANES;
   if (team < teams) {
+    // every fourth run's part asked for before the first of four is used; the running maximum as in the tiles
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    float den = 0.f;
-#pragma unroll 4
-    for (uint32_t c = c0 + team; c <= c1; c += teams)
-      if (there(c)) {
-        const float* p = piece(c);
-        const float f = exp2_fast(p[ml] - top);
-        const float4 x = *reinterpret_cast<const float4*>(p + r * D + lane * 4);
-        den = fmaf(p[ml + 1], f, den);
-        v.x = fmaf(x.x, f, v.x); v.y = fmaf(x.y, f, v.y); v.z = fmaf(x.z, f, v.z); v.w = fmaf(x.w, f, v.w);
+    float top = -FLT_MAX, den = 0.f;
+    for (uint32_t c = c0 + team; c <= c1; c += 4 * teams) {
+      float4 x[4];
+      float2 w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        w[i] = make_float2(-FLT_MAX, 0.f);
+        const uint32_t run = c + i * teams;
+        if (run <= c1 && there(run)) {
+          const float* p = piece(run);
+          w[i] = *reinterpret_cast<const float2*>(p + ml);
+          x[i] = *reinterpret_cast<const float4*>(p + r * D + lane * 4);
+        }
       }
+      const float now = fmaxf(fmaxf(fmaxf(w[0].x, w[1].x), fmaxf(w[2].x, w[3].x)), top), keep = exp2_fast(top - now);
+      top = now;
+      v.x *= keep; v.y *= keep; v.z *= keep; v.w *= keep;
+      den *= keep;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float f = exp2_fast(w[i].x - top);
+        den = fmaf(w[i].y, f, den);
+        v.x = fmaf(x[i].x, f, v.x); v.y = fmaf(x[i].y, f, v.y); v.z = fmaf(x[i].z, f, v.z); v.w = fmaf(x[i].w, f, v.w);
+      }
+    }
     *reinterpret_cast<float4*>(sums + team * D + lane * 4) = v;
-    if (lane == 0) dens[team] = den;
+    if (lane == 0) { tops[team] = top; dens[team] = den; }
   }
   __syncthreads();
   for (int j = tid; j < D; j += threads) {
-    float t = 0.f, l = 0.f;
-    for (int w = 0; w < teams; ++w) { t += sums[w * D + j]; l += dens[w]; }
+    float top = -FLT_MAX, t = 0.f, l = 0.f;
+    for (int w = 0; w < teams; ++w) top = fmaxf(top, tops[w]);
+    for (int w = 0; w < teams; ++w) {
+      const float f = exp2_fast(tops[w] - top);
+      t = fmaf(sums[w * D + j], f, t);
+      l = fmaf(dens[w], f, l);
+    }
     store_float(g.out, (uint64_t)s * g.cache.heads * D + (uint64_t)head * D + j, g.out_bf16, t / (l < FLT_MIN ? FLT_MIN : l));
   }
 }
@@ -658,8 +684,7 @@ cudaError_t attention_form(const AttnPagesArgs& g, void* scratch, int* launches,
       // a sequence's runs over as many teams as leave each a few
       constexpr int LANES = D / 4;
       const uint64_t each = c.runs / c.n;
-      int threads = (int)(each > 64 ? 512 : (each > 8 ? 256 : (each > 2 ? 128 : 64)));
-      if (threads < LANES) threads = LANES;
+      const int threads = each > 64 ? 1024 : (each > 16 ? 512 : (each > 4 ? 256 : 128));
       launch_pdl(attention_pages_join_kernel<D>, dim3((unsigned)(c.n < c.runs ? c.n : c.runs), g.cache.heads), dim3(threads),
                  threads / LANES * D * sizeof(float), stream, a);
       e = cudaGetLastError();

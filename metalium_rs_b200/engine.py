@@ -10,6 +10,7 @@ fallback -- without the built library, or without a B200, construction fails.
 from __future__ import annotations
 
 import ctypes as C
+import struct
 from dataclasses import dataclass
 from pathlib import Path
 from typing import Optional, Sequence, Tuple
@@ -119,6 +120,14 @@ def _prepare(_lib: C.CDLL) -> C.CDLL:
         _lib.b200_traffic_get.restype = None
         _lib.b200_last_oom.restype = None
         _lib.b200_release_trace.restype = None
+        # A step's calls: with their argument types declared they take plain numbers, at a third of the cost of wrapping each
+        u64, i32, u32, f32, p = C.c_uint64, C.c_int32, C.c_uint32, C.c_float, C.c_void_p
+        for name, types in (("b200_rope_append_pages", [p, p, p] + [u64] * 7 + [i32, i32, u64, p, p]),
+                            ("b200_attention_pages", [p, p, p] + [u64] * 4 + [u32, f32, i32, u64, p, p]),
+                            ("b200_token_logprobs", [p, u64, u64, f32, u32, p, p, p]),
+                            ("b200_token_logprobs_backward", [p] + [u64] * 6 + [f32, i32, u64, p, p])):
+            if hasattr(_lib, name):
+                getattr(_lib, name).argtypes = types
     return _lib
 
 
@@ -142,6 +151,16 @@ def _block(b) -> "BlockArg":
         return b
     bid, at, dims = b
     return BlockArg(bid, (C.c_uint64 * 2)(*at), (C.c_uint64 * 2)(*dims))
+
+
+_BLOCK = struct.Struct("=5Q")
+
+
+def _block_ptr(b):
+    """A block for a step's call: the bytes of a `BlockArg`, without making one."""
+    if isinstance(b, BlockArg):
+        return C.byref(b)
+    return _BLOCK.pack(b[0], *b[1], *b[2])
 
 
 Out = Tuple[int, Tuple[int, int]]
@@ -709,38 +728,34 @@ class CudaEngine:
         """RoPE on a projection's query and key heads and the cache write as one pass (`b200_rope_append_pages`): qkv is a
         block [n, (heads + 2 kv_heads) head_dim]; row i is the token at positions[i] of sequence sequences[i] (None: of
         sequence i), -1 a padding row.  Returns the rotated query heads, with `keys` the rotated key heads behind them."""
-        b = _block(qkv)
-        return self._call(self._lib.b200_rope_append_pages, C.byref(shape), C.byref(b), C.c_uint64(cos or 0), C.c_uint64(sin or 0),
-                          C.c_uint64(positions), C.c_uint64(sequences or 0), C.c_uint64(page_table), C.c_uint64(key_pages),
-                          C.c_uint64(value_pages), C.c_int32(1 if keys else 0), C.c_int32(1 if bf16 else 0), C.c_uint64(into))
+        return self._call(self._lib.b200_rope_append_pages, C.byref(shape), _block_ptr(qkv), cos or 0, sin or 0, positions, sequences or 0,
+                          page_table, key_pages, value_pages, 1 if keys else 0, 1 if bf16 else 0, into)
 
     def attention_pages(self, shape: "PageShape", q, key_pages: int, value_pages: int, page_table: int, positions: int, scale: float,
                         window: int = 0, bf16: bool = False, into: int = 0) -> Out:
         """One new token's attention over its sequence's pages (`b200_attention_pages`): q is a block
         [n, heads head_dim], row i the token at positions[i] of sequence i (-1: an idle slot, a row of zeros); `window` > 0
         keeps the last `window` positions.  Returns [n, heads head_dim]."""
-        b = _block(q)
-        return self._call(self._lib.b200_attention_pages, C.byref(shape), C.byref(b), C.c_uint64(key_pages), C.c_uint64(value_pages),
-                          C.c_uint64(page_table), C.c_uint64(positions), C.c_uint32(window), C.c_float(scale), C.c_int32(1 if bf16 else 0),
-                          C.c_uint64(into))
+        if not 0 <= window < 2**32:
+            raise ValueError("a window is 0 (every position) or a count of positions")
+        return self._call(self._lib.b200_attention_pages, C.byref(shape), _block_ptr(q), key_pages, value_pages, page_table, positions,
+                          window, scale, 1 if bf16 else 0, into)
 
     def token_logprobs(self, logits: int, ids: int, scale: float = 1.0, top: int = 0, into: Optional[Sequence[int]] = None):
         """(logprob, entropy, lse) [rows, 1] of the given tokens under softmax(scale * logits), and with `top` > 0 the
         (columns, log probabilities) [rows, top] of the largest logits (`b200_token_logprobs`): three or five (id, dims)."""
-        out = (C.c_uint64 * 5)()
-        dims = (C.c_uint64 * 2)()
-        dst = None
-        if into is not None:
-            dst = (C.c_uint64 * 5)(*into)
-        self._check(self._lib.b200_token_logprobs(self._e, C.c_uint64(logits), C.c_uint64(ids), C.c_float(scale), C.c_uint32(top), dst, out, dims))
+        if not 0 <= top < 2**32:
+            raise ValueError("the alternatives are a count")
+        out, dims = (C.c_uint64 * 5)(), (C.c_uint64 * 2)()
+        self._check(self._lib.b200_token_logprobs(self._e, logits, ids, scale, top, (C.c_uint64 * 5)(*into) if into is not None else None, out, dims))
         rows = dims[0]
         return [(out[i], (rows, 1 if i < 3 else top)) for i in range(5 if top else 3)]
 
     def token_logprobs_backward(self, logits: int, ids: int, lse: int, entropy: Optional[int], d_logprob: int, d_entropy: Optional[int] = None,
                                 scale: float = 1.0, bf16: bool = False, into: int = 0) -> Out:
         """The gradient of `token_logprobs`' log probabilities (and, with d_entropy, entropies) with respect to the logits."""
-        return self._call(self._lib.b200_token_logprobs_backward, C.c_uint64(logits), C.c_uint64(ids), C.c_uint64(lse), C.c_uint64(entropy or 0),
-                          C.c_uint64(d_logprob), C.c_uint64(d_entropy or 0), C.c_float(scale), C.c_int32(1 if bf16 else 0), C.c_uint64(into))
+        return self._call(self._lib.b200_token_logprobs_backward, logits, ids, lse, entropy or 0, d_logprob, d_entropy or 0, scale,
+                          1 if bf16 else 0, into)
 
     def set_matmul_sm_limit(self, sms: int):
         """Tensor-core products use at most `sms` SMs (0 = all): room for a collective beside them."""
