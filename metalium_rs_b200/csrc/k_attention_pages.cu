@@ -18,7 +18,7 @@
 // Precision: keys and values are the cache's own values.  The tensor cores' tile has sixteen rows, and a head takes two of
 // them: row r has an operand's leading part and row r + 8 the next one, so one product does both.  On the BF16 path an F32
 // query is three BF16 parts (exact) or, for a BF16 result, two (2^-16), and so is a probability; on the F32 path every operand
-// is two TF32 parts, of whose four products three are kept (2^-21).  For an F32 result a tile's products start from zero and are
+// is two TF32 parts (2^-22).  For an F32 result a tile's products start from zero and are
 // added to the running rows in F32; else the tensor cores accumulate them.
 #include <cfloat>
 #include <cmath>
@@ -36,7 +36,7 @@ namespace {
 template <typename KV, int D>
 struct Form {
   static constexpr bool BF = sizeof(KV) == 2;
-  static constexpr int WARPS = !BF && D > 128 ? 2 : 4;        // an F32 tile of a wide head is 33 KB a warp
+  static constexpr int WARPS = BF ? (D > 192 ? 3 : 4) : (D <= 96 ? 4 : (D == 192 ? 2 : 3));
   static constexpr int THREADS = WARPS * 32;
   // shared-memory row pitches that let eight rows (or the four position pairs of an F32 fragment) fall into distinct banks
   static constexpr int K_PITCH = D * (int)sizeof(KV) + (BF ? 16 : 32);
@@ -46,13 +46,8 @@ struct Form {
   // tile are REST, its pieces of a row PIECES
   static constexpr int CHUNKS = D * (int)sizeof(KV) / 16;     // 16-byte pieces of a row
   static constexpr int LANES = CHUNKS % 8 ? 4 : 8, ROWS = 32 / LANES, REST = 16 / ROWS, PIECES = CHUNKS / LANES;
-#ifndef ATTN_BLOCKS_128
-#define ATTN_BLOCKS_128 2
-#endif
-#ifndef ATTN_BLOCKS_64
-#define ATTN_BLOCKS_64 3
-#endif
-  static constexpr int BLOCKS = BF ? (D <= 64 ? ATTN_BLOCKS_64 : (D <= 128 ? ATTN_BLOCKS_128 : 1)) : (D <= 64 ? 2 : 1);
+  // blocks an SM: as many warps as their registers and two or three tiles each leave room for
+  static constexpr int BLOCKS = BF ? (D <= 64 ? 3 : 2) : (D <= 64 ? 3 : (D <= 192 ? 2 : 1));
   static __host__ __device__ int prefix_bytes(uint32_t n) { return (int)(((n + 1) * 4 + 127) / 128 * 128); }
 };
 constexpr uint32_t MAX_SEQUENCES = 512;  // a launch's; its prefix sums lie in shared memory
@@ -110,11 +105,9 @@ __device__ __forceinline__ void mma_tf32(float* c, uint32_t a0, uint32_t a1, uin
   asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ uint32_t tf32_of(float x) {
-  uint32_t r;
-  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r) : "f"(x));
-  return r;
-}
+// A value's leading TF32 part, cut, and what is left of it: exact, and a TF32 value but for its last two bits.
+__device__ __forceinline__ uint32_t tf32_of(float x) { return __float_as_uint(x) & 0xffffe000u; }
+__device__ __forceinline__ uint32_t tf32_rest(float x) { return __float_as_uint(x - __uint_as_float(tf32_of(x))); }
 __device__ __forceinline__ float exp2_fast(float x) {   // the hardware's 2^x: 2 units in the last place, 2^-inf = 0
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
@@ -381,13 +374,12 @@ __global__ void __launch_bounds__(Form<KV, D>::THREADS, Form<KV, D>::BLOCKS) att
 #pragma unroll
           for (int kk = 0; kk < D / 8; ++kk) {
             const uint32_t q0 = tf32_of(__uint_as_float(qf[kk][0])), q1 = tf32_of(__uint_as_float(qf[kk][1]));
-            const uint32_t p0 = __float_as_uint(__uint_as_float(qf[kk][0]) - __uint_as_float(q0)), p1 = __float_as_uint(__uint_as_float(qf[kk][1]) - __uint_as_float(q1));
+            const uint32_t p0 = tf32_rest(__uint_as_float(qf[kk][0])), p1 = tf32_rest(__uint_as_float(qf[kk][1]));
 #pragma unroll
             for (int nt = 0; nt < 2; ++nt) {
               const float2 k = lds2(k_at + (nt * 8 + gr) * F::K_PITCH + (kk * 8 + 2 * t4) * 4);
-              const uint32_t b0 = tf32_of(k.x), b1 = tf32_of(k.y);
-              mma_tf32(c[kk & 1][nt], q0, 0u, q1, 0u, __float_as_uint(k.x - __uint_as_float(b0)), __float_as_uint(k.y - __uint_as_float(b1)));
-              mma_tf32(c[kk & 1][nt], q0, p0, q1, p1, b0, b1);
+              mma_tf32(c[kk & 1][nt], q0, p0, q1, p1, tf32_rest(k.x), tf32_rest(k.y));
+              mma_tf32(c[kk & 1][nt], q0, p0, q1, p1, tf32_of(k.x), tf32_of(k.y));
             }
           }
 #pragma unroll
@@ -476,7 +468,7 @@ __global__ void __launch_bounds__(Form<KV, D>::THREADS, Form<KV, D>::BLOCKS) att
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
               hi[nt][e] = tf32_of(x[nt][e]);
-              lo[nt][e] = __float_as_uint(x[nt][e] - __uint_as_float(hi[nt][e]));
+              lo[nt][e] = tf32_rest(x[nt][e]);
             }
           const uint32_t vs = v_at + 2 * t4 * F::V_PITCH + gr * 4;
 #pragma unroll
@@ -486,9 +478,8 @@ __global__ void __launch_bounds__(Form<KV, D>::THREADS, Form<KV, D>::BLOCKS) att
             for (int nt = 0; nt < 2; ++nt) {
               const float u = lds1(vs + nt * 8 * F::V_PITCH + j * 32);
               const float v = lds1(vs + (nt * 8 + 1) * F::V_PITCH + j * 32);
-              const uint32_t b0 = tf32_of(u), b1 = tf32_of(v);
-              mma_tf32(c, hi[nt][0], 0u, hi[nt][1], 0u, __float_as_uint(u - __uint_as_float(b0)), __float_as_uint(v - __uint_as_float(b1)));
-              mma_tf32(c, hi[nt][0], lo[nt][0], hi[nt][1], lo[nt][1], b0, b1);
+              mma_tf32(c, hi[nt][0], lo[nt][0], hi[nt][1], lo[nt][1], tf32_rest(u), tf32_rest(v));
+              mma_tf32(c, hi[nt][0], lo[nt][0], hi[nt][1], lo[nt][1], tf32_of(u), tf32_of(v));
             }
             o[j][0] = fmaf(o[j][0], f, c[0] + c[2]);
             o[j][1] = fmaf(o[j][1], f, c[1] + c[3]);
