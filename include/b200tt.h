@@ -494,8 +494,8 @@ int32_t b200_attention_pages(b200_engine*, const b200_page_shape* shape, const b
  *                         equal values by the lower column, NaN above everything (`argmax_row`'s order), and their y - lse
  * One pass over the logits; sums in F32 under the row's maximum.  A row of -inf only has lse -inf, entropy 0 and log
  * probabilities -inf; a row with a NaN or +inf has NaN in all three.  Another id outside the columns sets DOMAIN (and gives 0).
- * `into` is NULL or five ids as `b200_rope_append_pages` takes one (0: a new buffer).  Refused unless scale is positive and
- * finite, top <= 32 and top <= vocab. */
+ * `into` is NULL or five ids as `b200_rope_append_pages` takes one (0: a new buffer).  Refused unless scale lies
+ * within 1e-20 .. 1e20, top <= 32 and top <= vocab. */
 int32_t b200_token_logprobs(b200_engine*, b200_buffer logits, b200_buffer ids, float scale, uint32_t top, const b200_buffer into[5],
                             b200_buffer out[5], uint64_t out_dims[2]);
 /* The gradient of the first two with respect to the logits: with p = exp(y - lse) and the rows' upstream gradients

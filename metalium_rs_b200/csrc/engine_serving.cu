@@ -97,7 +97,8 @@ int page_view(b200_engine* e, const b200_page_shape* shape, b200_buffer key_page
   return B200_OK;
 }
 
-bool good_scale(float s) { return std::isfinite(s) && s > 0.f; }
+// Within what an F32 logit times it can be told from -inf by.
+bool good_scale(float s) { return s >= 1e-20f && s <= 1e20f; }
 
 // `rows` F32 values as one row or one column (a per-row statistic or gradient).
 int row_values(b200_engine* e, b200_buffer id, uint64_t rows, Buf** b, const char* name, const char* what) {
@@ -221,7 +222,7 @@ int32_t b200_token_logprobs(b200_engine* e, b200_buffer logits, b200_buffer ids,
   const uint64_t rows = X->rows, cols = X->cols;
   st = int_list(e, ids, rows, &I, "ids", what);
   if (st) return st;
-  if (!good_scale(scale)) return e->fail(B200_UNSUPPORTED, "%s: the scale is positive and finite", what);
+  if (!good_scale(scale)) return e->fail(B200_UNSUPPORTED, "%s: the scale %g is not within 1e-20 .. 1e20", what, scale);
   if (top > 32 || top > cols) return e->fail(B200_UNSUPPORTED, "%s: the %u largest of %llu columns (at most 32)", what, top, (ull)cols);
   LogprobArgs g;
   g.logits = X->ptr; g.bf16 = X->elem == B200_BF16; g.rows = rows; g.cols = cols;
@@ -258,7 +259,7 @@ int32_t b200_token_logprobs_backward(b200_engine* e, b200_buffer logits, b200_bu
   if (!st && d_entropy) st = row_values(e, d_entropy, rows, &GH, "d_entropy", what);
   if (!st && d_entropy) st = row_values(e, entropy, rows, &H, "entropy", what);
   if (st) return st;
-  if (!good_scale(scale)) return e->fail(B200_UNSUPPORTED, "%s: the scale is positive and finite", what);
+  if (!good_scale(scale)) return e->fail(B200_UNSUPPORTED, "%s: the scale %g is not within 1e-20 .. 1e20", what, scale);
   std::vector<Span> spans = {span_of(X), span_of(I), span_of(L), span_of(G)};
   if (GH) { spans.push_back(span_of(GH)); spans.push_back(span_of(H)); }
   Result r;

@@ -27,9 +27,36 @@ __device__ __forceinline__ float exp2_fast(float x) {   // the hardware's 2^x: 2
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
-__device__ __forceinline__ float max_nan(float a, float b) {   // a NaN stays one
+// A product whose subnormal results are zero: a BF16 result below 2^-126 is stored as zero (`f32_to_bf16_bits`).
+__device__ __forceinline__ float mul_flush(float a, float b) {
   float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  asm("mul.ftz.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+// Two F32 operations an instruction.
+__device__ __forceinline__ uint64_t pair_of(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 floats_of(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
 
@@ -41,14 +68,30 @@ __device__ __forceinline__ uint64_t key_of(float v, uint32_t col) {
   return ((uint64_t)u << 32) | (uint32_t)~col;
 }
 __device__ __forceinline__ uint32_t col_of(uint64_t key) { return ~(uint32_t)key; }
+__device__ __forceinline__ float value_of(uint64_t key) {
+  const uint32_t u = (uint32_t)(key >> 32);
+  return __uint_as_float(u & 0x80000000u ? u & 0x7fffffffu : ~u);
+}
 
-template <typename T> struct Vec;        // a 16-byte piece of a row
+// A 16-byte piece of a row.  LOW: what -inf (and everything below) counts as in the sums, so that a term of 0 times its
+// exponent is 0; nothing above it is touched, a NaN stays one.
+constexpr float LOW = -1.0e30f;
+template <typename T> struct Vec;
 template <> struct Vec<float> {
   static constexpr int N = 4;
   static __device__ __forceinline__ float one(const float* p) { return *p; }
   static __device__ __forceinline__ void widen(const uint4& w, float* f) {
     f[0] = __uint_as_float(w.x); f[1] = __uint_as_float(w.y); f[2] = __uint_as_float(w.z); f[3] = __uint_as_float(w.w);
   }
+  static __device__ __forceinline__ float top(const uint4& w) {
+    return fmaxf(fmaxf(__uint_as_float(w.x), __uint_as_float(w.y)), fmaxf(__uint_as_float(w.z), __uint_as_float(w.w)));
+  }
+  static __device__ __forceinline__ float low(uint32_t w) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(__uint_as_float(w)), "f"(LOW));
+    return r;
+  }
+  static __device__ __forceinline__ void pairs(const uint4& w, uint64_t* v) { v[0] = pair_of(low(w.x), low(w.y)); v[1] = pair_of(low(w.z), low(w.w)); }
 };
 template <> struct Vec<uint16_t> {
   static constexpr int N = 8;
@@ -59,38 +102,29 @@ template <> struct Vec<uint16_t> {
     f[4] = __uint_as_float(w.z << 16); f[5] = __uint_as_float(w.z & 0xffff0000u);
     f[6] = __uint_as_float(w.w << 16); f[7] = __uint_as_float(w.w & 0xffff0000u);
   }
+  static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+  }
+  static __device__ __forceinline__ float top(const uint4& w) {
+    const uint32_t m = max2(max2(w.x, w.y), max2(w.z, w.w));
+    return fmaxf(__uint_as_float(m << 16), __uint_as_float(m & 0xffff0000u));
+  }
+  static __device__ __forceinline__ uint64_t low(uint32_t w) {
+    uint32_t r;
+    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(w), "r"(0xf14af14au));   // -1.0003e30 twice
+    return pair_of(__uint_as_float(r << 16), __uint_as_float(r & 0xffff0000u));
+  }
+  static __device__ __forceinline__ void pairs(const uint4& w, uint64_t* v) { v[0] = low(w.x); v[1] = low(w.y); v[2] = low(w.z); v[3] = low(w.w); }
 };
 
-// ---- sorted lists of 32 keys, one a lane, the largest first
-__device__ __forceinline__ uint64_t order_pair(uint64_t v, int lane, int apart, bool falling) {
-  const uint64_t o = __shfl_xor_sync(0xffffffffu, v, apart);
-  return ((lane & apart) == 0) == falling ? (v > o ? v : o) : (v < o ? v : o);
-}
-__device__ __forceinline__ uint64_t sort32(uint64_t v, int lane) {
-#pragma unroll
-  for (int k = 2; k <= 32; k <<= 1)
-#pragma unroll
-    for (int j = k / 2; j; j >>= 1) v = order_pair(v, lane, j, (lane & k) == 0);
-  return v;
-}
-// The largest 32 of two sorted lists: lane i's larger of a[i] and b[31 - i] is a bitonic list of them.
-__device__ __forceinline__ uint64_t merge32(uint64_t a, uint64_t b_reversed, int lane) {
-  uint64_t v = a > b_reversed ? a : b_reversed;
-#pragma unroll
-  for (int j = 16; j; j >>= 1) v = order_pair(v, lane, j, true);
-  return v;
-}
-
-// Sums under a maximum: m in units of log2, s = sum 2^(y - m), t = sum 2^(y - m) (y - m), y = x scale log2 e.
+// Sums under a reference m in units of log2: s = sum 2^(y - m), t = sum 2^(y - m) (y - m), y = x scale log2 e.
 struct Sums { float m, s, t; };
-__device__ __forceinline__ Sums under(const Sums& a, float m) {       // a's sums under another, larger maximum
+__device__ __forceinline__ Sums under(const Sums& a, float m) {       // a's sums under another reference
+  if (a.s == 0.f) return Sums{m, 0.f, 0.f};                           // nothing summed stays nothing, however far the reference moved
   const float d = a.m - m, f = exp2_fast(d);
-  return Sums{m, a.s * f, a.s == 0.f ? 0.f : f * fmaf(a.s, d, a.t)};  // nothing summed stays nothing, however far the maximum moved
-}
-__device__ __forceinline__ Sums both(const Sums& a, const Sums& b) {
-  const float m = fmaxf(a.m, b.m);
-  const Sums x = under(a, m), y = under(b, m);
-  return Sums{m, x.s + y.s, x.t + y.t};
+  return Sums{m, a.s * f, f * fmaf(a.s, d, a.t)};
 }
 
 // A block's slice of a row: 16-byte pieces from the address below its start, the pieces of thread i being i, i + THREADS, ...
@@ -110,33 +144,60 @@ template <typename T, int THREADS> struct Slice {
   }
   __device__ __forceinline__ uint4 raw(uint32_t u) const { return __ldg(reinterpret_cast<const uint4*>(row + origin) + u); }
   // a piece's values; those outside the slice are -inf
-  __device__ __forceinline__ void load(uint32_t u, float* x) const {
-    if (whole(u)) { Vec<T>::widen(raw(u), x); return; }
+  __device__ __forceinline__ uint4 piece(uint32_t u) const {
+    if (whole(u)) return raw(u);
+    uint32_t w[4];
 #pragma unroll
-    for (int e = 0; e < Vec<T>::N; ++e) {
-      const int64_t c = origin + (int64_t)u * Vec<T>::N + e;
-      x[e] = c >= first && c < last ? Vec<T>::one(row + c) : -INFINITY;
+    for (int i = 0; i < 4; ++i) {
+      w[i] = sizeof(T) == 2 ? 0xff80ff80u : 0xff800000u;
+#pragma unroll
+      for (int e = 0; e < 4 / (int)sizeof(T); ++e) {
+        const int64_t c = origin + (int64_t)u * Vec<T>::N + i * (4 / (int)sizeof(T)) + e;
+        if (c >= first && c < last) {
+          if constexpr (sizeof(T) == 2) w[i] = e ? (w[i] & 0xffffu) | ((uint32_t)row[c] << 16) : (w[i] & 0xffff0000u) | row[c];
+          else w[i] = __float_as_uint(row[c]);
+        }
+      }
     }
+    return make_uint4(w[0], w[1], w[2], w[3]);
   }
 };
 
-// One more group of a thread's values: its largest so far and the sums under it.
-template <int N>
-__device__ __forceinline__ void take(const float (&x)[N], float c, float& best, Sums& a) {
-  float top = x[0];
+// A thread's running state over its pieces: its largest value and the first piece that has it, and the sums.  The reference
+// follows the largest value only when that is 2^16 above it: within that, terms and sums keep their bits, and the step that
+// moves it (a thread meets four new maxima in 25 pieces, so one of a warp's threads meets one in almost every piece) stays rare.
+template <typename T> struct Running {
+  float best = -INFINITY, m = 0.f;
+  uint32_t piece;
+  uint64_t s[2] = {0, 0}, t[2] = {0, 0};
+  __device__ __forceinline__ void take(const uint4& w, uint32_t u, float c, uint64_t c2) {
+    const float top = Vec<T>::top(w), at = fmaf(top, c, -m);
+    if (at > 16.f || (best <= LOW && top > LOW)) move(fminf(fmaxf(top * c, -FLT_MAX), FLT_MAX));
+    piece = top > best ? u : piece;
+    best = fmaxf(best, top);
+    uint64_t v[Vec<T>::N / 2];
+    Vec<T>::pairs(w, v);
+    const uint64_t ref = pair_of(-m, -m);
 #pragma unroll
-  for (int e = 1; e < N; ++e) top = fmaxf(top, x[e]);
-  if (top > best) {
-    best = top;
-    a = under(a, fmaxf(top * c, -FLT_MAX));
+    for (int i = 0; i < Vec<T>::N / 2; ++i) {
+      const uint64_t z = fma2(v[i], c2, ref);
+      const float2 e = floats_of(z);
+      const uint64_t p = pair_of(exp2_fast(e.x), exp2_fast(e.y));
+      s[i & 1] = add2(s[i & 1], p);
+      t[i & 1] = fma2(p, z, t[i & 1]);
+    }
   }
-#pragma unroll
-  for (int e = 0; e < N; ++e) {
-    const float z = max_nan(fmaf(x[e], c, -a.m), -200.f), p = exp2_fast(z);
-    a.s += p;
-    a.t = fmaf(p, z, a.t);
+  __device__ __forceinline__ Sums sums() const {           // a thread with nothing above LOW has no reference
+    const float2 a = floats_of(add2(s[0], s[1])), b = floats_of(add2(t[0], t[1]));
+    return Sums{best > LOW ? m : -FLT_MAX, a.x + a.y, b.x + b.y};
   }
-}
+  __device__ __forceinline__ void move(float to) {
+    const Sums a = under(Sums{m, sums().s, sums().t}, to);
+    s[0] = pair_of(a.s, 0.f); t[0] = pair_of(a.t, 0.f);
+    s[1] = t[1] = 0;
+    m = to;
+  }
+};
 
 // The slice's `top` largest keys, one after another: for slices with a NaN or with more candidates than the list holds.
 template <typename T, int THREADS>
@@ -165,16 +226,25 @@ __device__ void slow_top(const Slice<T, THREADS>& sl, uint32_t top, uint64_t* li
   __syncthreads();
 }
 
+// How many of `n` keys are larger than `key`: its place in the sorted list (no two are equal).
+__device__ __forceinline__ uint32_t place_of(uint64_t key, const uint64_t* keys, uint32_t n) {
+  uint32_t k = 0;
+#pragma unroll 8
+  for (uint32_t i = 0; i < n; ++i) k += keys[i] > key;
+  return k;
+}
+
 // A row a block, or a row a cluster of blocks with a slice each (SHARED).  One pass keeps each thread's sums and its largest
-// value.  The `top` largest of the threads' largest bound the row's `top` largest from below, and only the threads that hold
-// them can hold one: their pieces alone are read again (from L2), what reaches the bound is listed, and the list is sorted.
+// value.  Every warp's few largest of those bound the row's `top` largest from below, and only the threads that reach the bound
+// can hold one: their pieces alone are read again (from L2), and what reaches the bound is listed and put in order.
 template <typename T, int THREADS, bool SHARED>
 __global__ void __launch_bounds__(THREADS) token_logprobs_kernel(const __grid_constant__ LogprobArgs g) {
-  constexpr int WARPS = THREADS / 32, N = Vec<T>::N, HELD = THREADS >= 256 ? 1024 : 512;
-  __shared__ uint64_t lists[WARPS][TOP], held[HELD], sh[WARPS], slices[SHARED ? CLUSTER : 1][TOP];
+  constexpr int WARPS = THREADS / 32, N = Vec<T>::N, HELD = THREADS * 8;
+  __shared__ uint64_t held[HELD], sh[WARPS], slices[SHARED ? CLUSTER * TOP : TOP], list[TOP];
   __shared__ Sums warp_sums[WARPS], slice_sums[SHARED ? CLUSTER : 1];
   __shared__ float warp_best[WARPS], slice_best[SHARED ? CLUSTER : 1];
-  __shared__ uint32_t count;
+  __shared__ uint32_t count, owner_count;
+  __shared__ uint16_t owners[THREADS];
   pdl_enter();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   uint32_t rank = 0, size = 1;
@@ -188,21 +258,16 @@ __global__ void __launch_bounds__(THREADS) token_logprobs_kernel(const __grid_co
   const int64_t cols = (int64_t)g.cols, seg = (cols + size - 1) / size;
   const Slice<T, THREADS> sl(row, rank * seg < cols ? rank * seg : cols, (rank + 1) * seg < cols ? (rank + 1) * seg : cols);
   const float c = g.scale * LOG2E;
-  if (tid == 0) count = 0;
+  const uint64_t c2 = pair_of(c, c);
+  const uint32_t top = g.top;
+  if (tid == 0) count = owner_count = 0;
+  if (tid < TOP) list[tid] = 0;
 
   // ---- the pass: four pieces of a thread asked for before the first is used; the slice's cut ends by themselves
-  Sums a{-FLT_MAX, 0.f, 0.f};
-  float best = -INFINITY;
+  Running<T> a;
+  a.piece = (uint32_t)tid;               // a thread whose values are all -inf has its first
   const uint32_t lo = sl.pieces && !sl.whole(0) ? 1u : 0u, hi = sl.pieces && !sl.whole(sl.pieces - 1) ? sl.pieces - 1 : sl.pieces;
-  uint32_t best_piece = (uint32_t)tid;   // the first piece that holds `best`
-  const auto edge = [&](uint32_t u) {
-    float x[N];
-    sl.load(u, x);
-    const float was = best;
-    take<N>(x, c, best, a);
-    if (best > was) best_piece = u;
-  };
-  if (lo && tid == 0) edge(0);
+  if (lo && tid == 0) a.take(sl.piece(0), 0, c, c2);
   for (uint32_t u = lo && tid == 0 ? THREADS : tid; u < hi; u += 4 * THREADS) {
     uint4 w[4];
 #pragma unroll
@@ -210,100 +275,107 @@ __global__ void __launch_bounds__(THREADS) token_logprobs_kernel(const __grid_co
       if (u + i * THREADS < hi) w[i] = sl.raw(u + i * THREADS);
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      if (u + i * THREADS < hi) {
-        float x[N];
-        Vec<T>::widen(w[i], x);
-        const float was = best;
-        take<N>(x, c, best, a);
-        if (best > was) best_piece = u + i * THREADS;
-      }
+      if (u + i * THREADS < hi) a.take(w[i], u + i * THREADS, c, c2);
   }
-  if (hi < sl.pieces && hi >= lo && sl.pieces > lo && tid == (int)(hi % THREADS)) edge(hi);
+  if (hi < sl.pieces && hi >= lo && sl.pieces > lo && tid == (int)(hi % THREADS)) a.take(sl.piece(hi), hi, c, c2);
 
-  // ---- the slice's sums
-  Sums all = a;
-  float high = best;
+  // ---- the slice's sums: under the largest reference of the warp, then of the block
+  Sums all = a.sums();
+  float high = a.best;
+  {
+    float m = all.m;
 #pragma unroll
-  for (int o = 16; o; o >>= 1) {
-    const Sums b{__shfl_xor_sync(0xffffffffu, all.m, o), __shfl_xor_sync(0xffffffffu, all.s, o), __shfl_xor_sync(0xffffffffu, all.t, o)};
-    all = both(all, b);
-    high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, o));
+    for (int o = 16; o; o >>= 1) { m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o)); high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, o)); }
+    all = under(all, m);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) { all.s += __shfl_xor_sync(0xffffffffu, all.s, o); all.t += __shfl_xor_sync(0xffffffffu, all.t, o); }
   }
   if (lane == 0) { warp_sums[warp] = all; warp_best[warp] = high; }
-  const uint32_t top = g.top;
   const uint32_t threads = sl.pieces < (uint32_t)THREADS ? sl.pieces : (uint32_t)THREADS;   // those that hold a piece
+  uint64_t mine = 0;                     // this thread's largest key
   if (top && threads >= top) {
-    uint64_t key = 0;
     if (tid < (int)sl.pieces) {
-      // the lowest column of the piece with that value; a thread whose values are all -inf has its first
       float x[N];
-      sl.load(best_piece, x);
+      Vec<T>::widen(sl.piece(a.piece), x);
       int at = -1;
 #pragma unroll
       for (int e = N - 1; e >= 0; --e) {
-        const int64_t col = sl.origin + (int64_t)best_piece * N + e;
-        if (x[e] == best && col >= sl.first && col < sl.last) at = e;
+        const int64_t col = sl.origin + (int64_t)a.piece * N + e;
+        if (x[e] == a.best && col >= sl.first && col < sl.last) at = e;
       }
-      key = at < 0 ? 0 : key_of(best, (uint32_t)(sl.origin + (int64_t)best_piece * N + at));
+      if (at >= 0) mine = key_of(a.best, (uint32_t)(sl.origin + (int64_t)a.piece * N + at));
     }
-    lists[warp][lane] = sort32(key, lane);
+    // the `each`th largest of a warp whose threads all hold a piece, `each` such a warp's share of `top` (with no such warp, the
+    // first's `top`th: it has as many)
+    const uint32_t whole = threads < 32 ? 1 : threads / 32, each = (top + whole - 1) / whole;
+    uint64_t left = mine, last = 0;
+    for (uint32_t k = 0; k < each; ++k) {
+      const uint32_t h = __reduce_max_sync(0xffffffffu, (uint32_t)(left >> 32));
+      const uint32_t l = __reduce_max_sync(0xffffffffu, (uint32_t)(left >> 32) == h ? (uint32_t)left : 0u);
+      last = ((uint64_t)h << 32) | l;
+      if (left == last) left = 0;
+    }
+    if (lane == 0) sh[warp] = warp < (int)whole ? last : ~0ull;
   }
   __syncthreads();
-  all = warp_sums[0];
-  high = warp_best[0];
-  for (int w = 1; w < WARPS; ++w) { all = both(all, warp_sums[w]); high = fmaxf(high, warp_best[w]); }
+  {
+    float m = -FLT_MAX;
+    high = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) { m = fmaxf(m, warp_sums[w].m); high = fmaxf(high, warp_best[w]); }
+    all = Sums{m, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) {
+      const Sums b = under(warp_sums[w], m);
+      all.s += b.s;
+      all.t += b.t;
+    }
+  }
 
   // ---- the slice's largest
   if (top) {
     bool slow = all.s != all.s;          // a NaN or +inf: the maxima above passed over it
-    uint64_t bound = 0;
-    if (!slow && threads >= top) {
-#pragma unroll
-      for (int half = WARPS / 2; half; half >>= 1) {
-        uint64_t v = 0;
-        if (warp < half) v = merge32(lists[warp][lane], lists[warp + half][31 - lane], lane);
-        __syncthreads();
-        if (warp < half) lists[warp][lane] = v;
-        __syncthreads();
-      }
-      bound = lists[0][top - 1];
-    }
     if (!slow) {
-      const uint32_t each = (sl.pieces + THREADS - 1) / THREADS, owners = threads >= top ? top : threads;
-      for (uint32_t i = tid; i < owners * each; i += THREADS) {
-        const uint32_t o = i / each;
-        const uint32_t owner = threads >= top ? (uint32_t)(((int64_t)col_of(lists[0][o]) - sl.origin) / N % THREADS) : o;
-        const uint32_t u = owner + i % each * THREADS;
+      const bool bounded = threads >= top;
+      uint64_t bound = bounded ? sh[0] : 0;
+      if (bounded) {
+#pragma unroll
+        for (int w = 1; w < WARPS; ++w) bound = sh[w] < bound ? sh[w] : bound;
+      }
+      const float reach = value_of(bound);
+      // the threads that reach it (all that hold a piece, where there are fewer than `top` of those)
+      if (tid < (int)threads && mine >= bound) owners[atomicAdd(&owner_count, 1u)] = (uint16_t)tid;
+      __syncthreads();
+      const uint32_t each = (sl.pieces + THREADS - 1) / THREADS, n = owner_count * each;
+      for (uint32_t i = tid; i < n; i += THREADS) {
+        const uint32_t u = owners[i / each] + i % each * THREADS;
         if (u < sl.pieces) {
+          const uint4 w = sl.piece(u);
+          if (bounded && Vec<T>::top(w) < reach) continue;   // nearly all
           float x[N];
-          sl.load(u, x);
+          Vec<T>::widen(w, x);
 #pragma unroll
           for (int e = 0; e < N; ++e) {
             const int64_t col = sl.origin + (int64_t)u * N + e;
-            if (col >= sl.first && col < sl.last) {
-              const uint64_t key = key_of(x[e], (uint32_t)col);
-              if (key >= bound) {
-                const uint32_t k = atomicAdd(&count, 1u);
-                if (k < (uint32_t)HELD) held[k] = key;
-              }
+            const uint64_t key = key_of(x[e], (uint32_t)col);
+            if (key >= bound && col >= sl.first && col < sl.last) {
+              const uint32_t k = atomicAdd(&count, 1u);
+              if (k < (uint32_t)HELD) held[k] = key;
             }
           }
         }
       }
       __syncthreads();
       slow = count > (uint32_t)HELD;
+      // the list's order depends on the atomics, its keys do not
+      if (!slow)
+        for (uint32_t i = tid; i < count; i += THREADS) {
+          const uint64_t key = held[i];
+          const uint32_t k = place_of(key, held, count);
+          if (k < top) list[k] = key;
+        }
     }
-    if (slow) {
-      slow_top(sl, top, lists[0], sh);
-    } else if (warp == 0) {
-      // the list's order depends on the atomics, its keys do not, and no two are equal
-      uint64_t v = 0;
-      for (uint32_t i = 0; i < count; i += 32) {
-        const uint64_t x = sort32(i + lane < count ? held[i + lane] : 0, lane);
-        v = i ? merge32(v, __shfl_sync(0xffffffffu, x, 31 - lane), lane) : x;
-      }
-      lists[0][lane] = v;
-    }
+    if (slow) slow_top(sl, top, list, sh);
     __syncthreads();
   }
 
@@ -322,26 +394,36 @@ __global__ void __launch_bounds__(THREADS) token_logprobs_kernel(const __grid_co
       asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(at + 8), "f"(all.t) : "memory");
       asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(there(&slice_best[rank])), "f"(high) : "memory");
     }
-    if (top && warp == 0) asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(there(&slices[rank][lane])), "l"(lists[0][lane]) : "memory");
+    if (tid < (int)top) asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(there(&slices[rank * top + tid])), "l"(list[tid]) : "memory");
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
     if (rank) return;
-    all = slice_sums[0];
-    high = slice_best[0];
-    for (uint32_t w = 1; w < size; ++w) { all = both(all, slice_sums[w]); high = fmaxf(high, slice_best[w]); }
-    if (top && warp == 0) {
-      uint64_t v = slices[0][lane];
-      for (uint32_t w = 1; w < size; ++w) v = merge32(v, slices[w][31 - lane], lane);
-      lists[0][lane] = v;
+    float m = -FLT_MAX;
+    high = -INFINITY;
+    for (uint32_t w = 0; w < size; ++w) { m = fmaxf(m, slice_sums[w].m); high = fmaxf(high, slice_best[w]); }
+    all = Sums{m, 0.f, 0.f};
+    for (uint32_t w = 0; w < size; ++w) {
+      const Sums b = under(slice_sums[w], m);
+      all.s += b.s;
+      all.t += b.t;
+    }
+    if (top) {
+      for (uint32_t i = tid; i < size * top; i += THREADS) {
+        const uint64_t key = slices[i];
+        const uint32_t k = key ? place_of(key, slices, size * top) : top;    // 0: a slice with fewer values
+        if (k < top) list[k] = key;
+      }
+      __syncthreads();
     }
   }
 
   // y - lse and the statistics.  The pass's terms are 2^(x c - fl(high c)): the reference's rounding cancels in the results, but it
   // is a factor of up to 2^(|high c| 2^-24) on every term, and a product may leave the type's range (a row masked by the type's
-  // lowest value).  Rows with a reference from 1e8 on are taken again from differences to their largest.
+  // lowest value).  Rows with a reference from 1e8 on, or nothing above LOW, are taken again from differences to their largest.
+  if (high == INFINITY) all.s = NAN;
   float ref = all.m * LN2, log_sum = logf(all.s), entropy = log_sum - LN2 * all.t / all.s;
   const bool none = high == -INFINITY && all.s == 0.f;     // -inf only
-  const bool plain = none || !(fabsf(high) <= FLT_MAX) || fabsf(high * c) < 1e8f;
+  const bool plain = none || !(fabsf(high) <= FLT_MAX) || (fabsf(high * c) < 1e8f && high > LOW);
   if (none) { ref = -INFINITY; log_sum = 0.f; entropy = 0.f; }
   if (!plain) {
     float s = 0.f, t = 0.f;
@@ -374,7 +456,7 @@ __global__ void __launch_bounds__(THREADS) token_logprobs_kernel(const __grid_co
     g.logprob[r] = lp;
   }
   if (warp == 0 && lane < (int)top) {
-    const uint32_t col = col_of(lists[0][lane]);
+    const uint32_t col = col_of(list[lane]);
     g.top_ids[r * top + lane] = (int32_t)col;
     g.top_logprobs[r * top + lane] = (int64_t)col < cols ? log_prob(Vec<T>::one(row + col)) : -INFINITY;
   }
@@ -382,38 +464,45 @@ __global__ void __launch_bounds__(THREADS) token_logprobs_kernel(const __grid_co
 
 // scale (g (1[j = id] - p) - h p (y - lse + H)) with p = e^(y - lse).  Both types are read and written in groups of eight
 // elements of the whole matrix, whose ends are the result's 16-byte boundaries whatever the row's length; a group that two rows
-// share is written by both, an element at a time.  A row's segment of GROUPS * THREADS groups a block, all of a thread's groups
-// asked for before the first is used.
-constexpr int GROUPS = 2;
-// A product whose subnormal results are zero: a BF16 result below 2^-126 is stored as zero (`f32_to_bf16_bits`).
-__device__ __forceinline__ float mul_flush(float a, float b) {
-  float r;
-  asm("mul.ftz.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ void load_group(const LogprobGradArgs& g, uint64_t at, bool vec, float* x) {
-  if (g.bf16) {
+// share is written by both, an element at a time.  A block takes SEGMENT groups a thread of one row.
+constexpr int SEGMENT = 8;
+// A group's values, and the LOW of the sums above in place of -inf: 0 times its exponent is 0.
+template <bool BF, bool ENTROPY>
+__device__ __forceinline__ void load_group(const LogprobGradArgs& g, uint64_t at, int vec, uint64_t* v) {
+  if constexpr (BF) {
     const uint16_t* p = reinterpret_cast<const uint16_t*>(g.logits) + at;
-    if (vec) { Vec<uint16_t>::widen(__ldg(reinterpret_cast<const uint4*>(p)), x); return; }
+    uint4 w;
+    if (vec) w = __ldg(reinterpret_cast<const uint4*>(p));
+    else w = make_uint4(p[0] | (uint32_t)p[1] << 16, p[2] | (uint32_t)p[3] << 16, p[4] | (uint32_t)p[5] << 16, p[6] | (uint32_t)p[7] << 16);
+    if constexpr (ENTROPY) Vec<uint16_t>::pairs(w, v);
+    else {
+      float x[8];
+      Vec<uint16_t>::widen(w, x);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = bf16_bits_to_f32(p[e]);
+      for (int i = 0; i < 4; ++i) v[i] = pair_of(x[2 * i], x[2 * i + 1]);
+    }
   } else {
     const float* p = reinterpret_cast<const float*>(g.logits) + at;
-    if (vec) {
-      Vec<float>::widen(__ldg(reinterpret_cast<const uint4*>(p)), x);
-      Vec<float>::widen(__ldg(reinterpret_cast<const uint4*>(p) + 1), x + 4);
-      return;
+    uint4 w[2];
+    if (vec) { w[0] = __ldg(reinterpret_cast<const uint4*>(p)); w[1] = __ldg(reinterpret_cast<const uint4*>(p) + 1); }
+    else {
+      const uint32_t* q = reinterpret_cast<const uint32_t*>(p);
+      w[0] = make_uint4(q[0], q[1], q[2], q[3]); w[1] = make_uint4(q[4], q[5], q[6], q[7]);
     }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = p[e];
+    if constexpr (ENTROPY) { Vec<float>::pairs(w[0], v); Vec<float>::pairs(w[1], v + 2); }
+    else {
+      v[0] = pair_of(__uint_as_float(w[0].x), __uint_as_float(w[0].y)); v[1] = pair_of(__uint_as_float(w[0].z), __uint_as_float(w[0].w));
+      v[2] = pair_of(__uint_as_float(w[1].x), __uint_as_float(w[1].y)); v[3] = pair_of(__uint_as_float(w[1].z), __uint_as_float(w[1].w));
+    }
   }
 }
-template <bool ENTROPY>
+template <bool BF, bool OUT_BF, bool ENTROPY>
 __global__ void __launch_bounds__(256) token_logprobs_backward_kernel(const __grid_constant__ LogprobGradArgs g, uint32_t segments, int vec) {
+  constexpr int AHEAD = BF ? 4 : 2;      // groups asked for before the first is used: 64 bytes a thread
   pdl_enter();
   const uint64_t r = blockIdx.x / segments, base = r * g.cols, end = base + g.cols;
-  const uint64_t group0 = base / 8 + (uint64_t)(blockIdx.x % segments) * GROUPS * blockDim.x + threadIdx.x;
-  const float lse = g.lse[r], h = ENTROPY ? g.d_entropy[r] * g.scale : 0.f, H = ENTROPY ? g.entropy[r] : 0.f;
+  const uint64_t first = base / 8 + (uint64_t)(blockIdx.x % segments) * SEGMENT * blockDim.x + threadIdx.x;
+  const float lse = g.lse[r], h = ENTROPY ? -g.d_entropy[r] * g.scale : 0.f, H = ENTROPY ? g.entropy[r] : 0.f;
   int64_t id = g.ids[r];
   if (id < -1 || id >= (int64_t)g.cols) {
     if (threadIdx.x == 0) atomicCAS(g.err, 0, DOMAIN_ERROR);
@@ -422,28 +511,17 @@ __global__ void __launch_bounds__(256) token_logprobs_backward_kernel(const __gr
   const float up = id >= 0 ? g.d_logprob[r] * g.scale : 0.f;
   const uint64_t hot = id >= 0 ? base + (uint64_t)id : ~0ull;
   const bool empty = lse == -INFINITY;
-  float x[GROUPS][8];
-#pragma unroll
-  for (int i = 0; i < GROUPS; ++i) {
-    const uint64_t at = (group0 + (uint64_t)i * blockDim.x) * 8;
-    if (at >= base && at + 8 <= end) load_group(g, at, vec, x[i]);
-    else
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        x[i][e] = at + e >= base && at + e < end ? (g.bf16 ? bf16_bits_to_f32(reinterpret_cast<const uint16_t*>(g.logits)[at + e])
-                                                           : reinterpret_cast<const float*>(g.logits)[at + e]) : 0.f;
-  }
-#pragma unroll
-  for (int i = 0; i < GROUPS; ++i) {
-    const uint64_t at = (group0 + (uint64_t)i * blockDim.x) * 8;
-    if (at >= end) break;
-    float v[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float z = fmaf(x[i][e], g.scale, -lse), p = exp2_fast(z * LOG2E);
-      // an entry of -inf has p = 0 (as everything below -126 log 2 has): its z is kept finite so that their product is 0
-      v[e] = mul_flush(p, ENTROPY ? -(up + h * (fmaxf(z, -200.f) + H)) : -up);
-    }
+  const uint64_t scale2 = pair_of(g.scale, g.scale), lse2 = pair_of(-lse, -lse), log2e2 = pair_of(LOG2E, LOG2E);
+  const uint64_t h2 = pair_of(h, h), base2 = ENTROPY ? pair_of(fmaf(h, H, -up), fmaf(h, H, -up)) : pair_of(-up, -up);
+  // p (h (z + H) - up), z = y - lse
+  const auto value = [&](uint64_t x, float& v0, float& v1) {
+    const uint64_t z = fma2(x, scale2, lse2);
+    const float2 e = floats_of(mul2(z, log2e2));
+    const float2 k = floats_of(ENTROPY ? fma2(z, h2, base2) : base2);
+    v0 = mul_flush(exp2_fast(e.x), k.x);
+    v1 = mul_flush(exp2_fast(e.y), k.y);
+  };
+  const auto patch = [&](uint64_t at, float (&v)[8]) {       // the given token's own term, and a row of -inf only
     if (hot - at < 8)
 #pragma unroll
       for (int e = 0; e < 8; ++e)
@@ -451,24 +529,64 @@ __global__ void __launch_bounds__(256) token_logprobs_backward_kernel(const __gr
     if (empty)
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] = 0.f;
-    if (at >= base && at + 8 <= end) {
-      if (g.out_bf16) {
-        uint32_t w[4];
+  };
+  const auto put = [&](uint64_t at, const float (&v)[8]) {
+    if constexpr (OUT_BF) {
+      uint32_t w[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w[e]) : "f"(v[2 * e + 1]), "f"(v[2 * e]));
-        *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(g.out) + at) = make_uint4(w[0], w[1], w[2], w[3]);
-      } else {
-        float4* o = reinterpret_cast<float4*>(reinterpret_cast<float*>(g.out) + at);
-        o[0] = make_float4(v[0], v[1], v[2], v[3]);
-        o[1] = make_float4(v[4], v[5], v[6], v[7]);
-      }
+      for (int e = 0; e < 4; ++e) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w[e]) : "f"(v[2 * e + 1]), "f"(v[2 * e]));
+      *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(g.out) + at) = make_uint4(w[0], w[1], w[2], w[3]);
     } else {
+      float4* o = reinterpret_cast<float4*>(reinterpret_cast<float*>(g.out) + at);
+      o[0] = make_float4(v[0], v[1], v[2], v[3]);
+      o[1] = make_float4(v[4], v[5], v[6], v[7]);
+    }
+  };
+  // the block's groups; all of them inside the row but for its first and last segment
+  const uint64_t begin = first - threadIdx.x, stop = begin + (uint64_t)SEGMENT * blockDim.x;
+  const bool inner = begin * 8 >= base && stop * 8 <= end;
+  const bool plain = !empty && (hot < begin * 8 || hot >= stop * 8);
+#pragma unroll 1
+  for (int step = 0; step < SEGMENT; step += AHEAD) {
+    const uint64_t at0 = (first + (uint64_t)step * blockDim.x) * 8, apart = (uint64_t)blockDim.x * 8;
+    if (inner) {
+      uint64_t x[AHEAD][4];
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (at + e >= base && at + e < end) {
-          if (g.out_bf16) reinterpret_cast<uint16_t*>(g.out)[at + e] = f32_to_bf16_bits(__float_as_uint(v[e]));
-          else reinterpret_cast<float*>(g.out)[at + e] = v[e];
+      for (int i = 0; i < AHEAD; ++i) load_group<BF, ENTROPY>(g, at0 + i * apart, vec, x[i]);
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i) {
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) value(x[i][e], v[2 * e], v[2 * e + 1]);
+        if (!plain) patch(at0 + i * apart, v);
+        put(at0 + i * apart, v);
+      }
+      continue;
+    }
+    for (int i = 0; i < AHEAD; ++i) {
+      const uint64_t at = at0 + i * apart;
+      if (at >= end) break;
+      if (at >= base && at + 8 <= end) {
+        uint64_t x[4];
+        load_group<BF, ENTROPY>(g, at, vec, x);
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) value(x[e], v[2 * e], v[2 * e + 1]);
+        patch(at, v);
+        put(at, v);
+      } else {                                               // a group that this row shares with another
+        for (int e = 0; e < 8; ++e) {
+          if (at + e < base || at + e >= end) continue;
+          float y = BF ? bf16_bits_to_f32(reinterpret_cast<const uint16_t*>(g.logits)[at + e]) : reinterpret_cast<const float*>(g.logits)[at + e];
+          if (y < LOW) y = LOW;
+          float v, other;
+          value(pair_of(y, y), v, other);
+          if (at + e == hot) v += up;
+          if (empty) v = 0.f;
+          if constexpr (OUT_BF) reinterpret_cast<uint16_t*>(g.out)[at + e] = f32_to_bf16_bits(__float_as_uint(v));
+          else reinterpret_cast<float*>(g.out)[at + e] = v;
         }
+      }
     }
   }
 }
@@ -511,12 +629,19 @@ cudaError_t launch_token_logprobs_backward(const LogprobGradArgs& g, cudaStream_
   if (g.rows == 0) return cudaSuccess;
   const uint64_t groups = (g.cols + 7) / 8 + 1;            // a row that starts inside a group touches one more
   unsigned threads = 32;
-  while (threads < 256 && threads * GROUPS < groups) threads *= 2;
-  const uint64_t segments = (groups + threads * GROUPS - 1) / (threads * GROUPS), blocks = segments * g.rows;
+  while (threads < 256 && threads * SEGMENT < groups) threads *= 2;
+  const uint64_t segments = (groups + threads * SEGMENT - 1) / (threads * SEGMENT), blocks = segments * g.rows;
   if (blocks > 0x7fffffffull) return cudaErrorNotSupported;
   const int vec = (reinterpret_cast<uintptr_t>(g.logits) & 15) == 0;
-  launch_pdl(g.d_entropy ? token_logprobs_backward_kernel<true> : token_logprobs_backward_kernel<false>, dim3((unsigned)blocks), dim3(threads), 0, stream,
-             g, (uint32_t)segments, vec);
+  const auto go = [&](auto kernel) { launch_pdl(kernel, dim3((unsigned)blocks), dim3(threads), 0, stream, g, (uint32_t)segments, vec); };
+  const bool h = g.d_entropy != nullptr;
+  if (g.bf16) {
+    if (g.out_bf16) h ? go(token_logprobs_backward_kernel<true, true, true>) : go(token_logprobs_backward_kernel<true, true, false>);
+    else h ? go(token_logprobs_backward_kernel<true, false, true>) : go(token_logprobs_backward_kernel<true, false, false>);
+  } else {
+    if (g.out_bf16) h ? go(token_logprobs_backward_kernel<false, true, true>) : go(token_logprobs_backward_kernel<false, true, false>);
+    else h ? go(token_logprobs_backward_kernel<false, false, true>) : go(token_logprobs_backward_kernel<false, false, false>);
+  }
   return cudaGetLastError();
 }
 

@@ -173,7 +173,7 @@ def test_logprob_dims_and_refusals(e):
     assert [d for _, d in got] == [(5, 1)] * 3 and all(e.dims_of(i) == ((5, 1), F32) for i, _ in got)
     got = e.token_logprobs(zeros(e, 5, 100, BF16), e.reshape(ids, 1, 5)[0], 0.5, 32)
     assert [e.dims_of(i) for i, _ in got[3:]] == [((5, 32), I32), ((5, 32), F32)]
-    for k in (dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")), dict(scale=float("inf")), dict(top=33)):
+    for k in (dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")), dict(scale=float("inf")), dict(scale=1e-21), dict(top=33)):
         refused(lambda: e.token_logprobs(x, ids, **k))
     refused(lambda: e.token_logprobs(zeros(e, 5, 4), ids, top=5))
     refused(lambda: e.token_logprobs(zeros(e, 5, 100, I32), ids))
