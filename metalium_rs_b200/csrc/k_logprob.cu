@@ -68,7 +68,8 @@ __device__ __forceinline__ uint64_t key_of(float v, uint32_t col) {
   return ((uint64_t)u << 32) | (uint32_t)~col;
 }
 __device__ __forceinline__ uint32_t col_of(uint64_t key) { return ~(uint32_t)key; }
-__device__ __forceinline__ float value_of(uint64_t key) {
+__device__ __forceinline__ float value_of(uint64_t key) {      // 0, no key: below every value
+  if (key == 0) return -INFINITY;
   const uint32_t u = (uint32_t)(key >> 32);
   return __uint_as_float(u & 0x80000000u ? u & 0x7fffffffu : ~u);
 }
@@ -163,17 +164,19 @@ template <typename T, int THREADS> struct Slice {
   }
 };
 
-// A thread's running state over its pieces: its largest value and the first piece that has it, and the sums.  The reference
+// A thread's running state over its pieces: its largest value and the first piece that has it, the largest of the others, and
+// the sums.  The reference
 // follows the largest value only when that is 2^16 above it: within that, terms and sums keep their bits, and the step that
 // moves it (a thread meets four new maxima in 25 pieces, so one of a warp's threads meets one in almost every piece) stays rare.
 template <typename T> struct Running {
-  float best = -INFINITY, m = 0.f;
+  float best = -INFINITY, second = -INFINITY, m = 0.f;
   uint32_t piece;
   uint64_t s[2] = {0, 0}, t[2] = {0, 0};
   __device__ __forceinline__ void take(const uint4& w, uint32_t u, float c, uint64_t c2) {
     const float top = Vec<T>::top(w), at = fmaf(top, c, -m);
     if (at > 16.f || (best <= LOW && top > LOW)) move(fminf(fmaxf(top * c, -FLT_MAX), FLT_MAX));
     piece = top > best ? u : piece;
+    second = fmaxf(second, fminf(top, best));
     best = fmaxf(best, top);
     uint64_t v[Vec<T>::N / 2];
     Vec<T>::pairs(w, v);
@@ -235,8 +238,10 @@ __device__ __forceinline__ uint32_t place_of(uint64_t key, const uint64_t* keys,
 }
 
 // A row a block, or a row a cluster of blocks with a slice each (SHARED).  One pass keeps each thread's sums and its largest
-// value.  Every warp's few largest of those bound the row's `top` largest from below, and only the threads that reach the bound
-// can hold one: their pieces alone are read again (from L2), and what reaches the bound is listed and put in order.
+// value.  Every warp's few largest of those bound the row's `top` largest from below: a thread that reaches the bound reads the
+// piece of its largest again, and only where another of its pieces reaches it too (one thread in ten of those) are all of that
+// thread's read by the block.  What reaches the bound is listed and put in order.  Where that is more than the list holds -- rows
+// of few distinct values -- the bound is taken again from keys, by value and column.
 template <typename T, int THREADS, bool SHARED>
 __global__ void __launch_bounds__(THREADS) token_logprobs_kernel(const __grid_constant__ LogprobArgs g) {
   constexpr int WARPS = THREADS / 32, N = Vec<T>::N, HELD = THREADS * 8;
@@ -245,6 +250,7 @@ __global__ void __launch_bounds__(THREADS) token_logprobs_kernel(const __grid_co
   __shared__ float warp_best[WARPS], slice_best[SHARED ? CLUSTER : 1];
   __shared__ uint32_t count, owner_count;
   __shared__ uint16_t owners[THREADS];
+  __shared__ uint32_t done[THREADS];
   pdl_enter();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   uint32_t rank = 0, size = 1;
@@ -262,6 +268,9 @@ __global__ void __launch_bounds__(THREADS) token_logprobs_kernel(const __grid_co
   const uint32_t top = g.top;
   if (tid == 0) count = owner_count = 0;
   if (tid < TOP) list[tid] = 0;
+  const int32_t id = g.ids[r];
+  const bool named = id >= 0 && id < cols;
+  const float id_logit = named ? Vec<T>::one(row + id) : 0.f;
 
   // ---- the pass: four pieces of a thread asked for before the first is used; the slice's cut ends by themselves
   Running<T> a;
@@ -292,23 +301,12 @@ __global__ void __launch_bounds__(THREADS) token_logprobs_kernel(const __grid_co
   }
   if (lane == 0) { warp_sums[warp] = all; warp_best[warp] = high; }
   const uint32_t threads = sl.pieces < (uint32_t)THREADS ? sl.pieces : (uint32_t)THREADS;   // those that hold a piece
-  uint64_t mine = 0;                     // this thread's largest key
-  if (top && threads >= top) {
-    if (tid < (int)sl.pieces) {
-      float x[N];
-      Vec<T>::widen(sl.piece(a.piece), x);
-      int at = -1;
-#pragma unroll
-      for (int e = N - 1; e >= 0; --e) {
-        const int64_t col = sl.origin + (int64_t)a.piece * N + e;
-        if (x[e] == a.best && col >= sl.first && col < sl.last) at = e;
-      }
-      if (at >= 0) mine = key_of(a.best, (uint32_t)(sl.origin + (int64_t)a.piece * N + at));
-    }
-    // the `each`th largest of a warp whose threads all hold a piece, `each` such a warp's share of `top` (with no such warp, the
-    // first's `top`th: it has as many)
-    const uint32_t whole = threads < 32 ? 1 : threads / 32, each = (top + whole - 1) / whole;
-    uint64_t left = mine, last = 0;
+  const bool bounded = threads >= top;
+  // the `each`th largest of a warp whose threads all hold a piece, `each` such a warp's share of `top` (with no such warp, the
+  // first's `top`th: it has as many)
+  const uint32_t whole = threads < 32 ? 1 : threads / 32, each = (top + whole - 1) / whole;
+  const auto bound_warp = [&](uint64_t left) {
+    uint64_t last = 0;
     for (uint32_t k = 0; k < each; ++k) {
       const uint32_t h = __reduce_max_sync(0xffffffffu, (uint32_t)(left >> 32));
       const uint32_t l = __reduce_max_sync(0xffffffffu, (uint32_t)(left >> 32) == h ? (uint32_t)left : 0u);
@@ -316,7 +314,9 @@ __global__ void __launch_bounds__(THREADS) token_logprobs_kernel(const __grid_co
       if (left == last) left = 0;
     }
     if (lane == 0) sh[warp] = warp < (int)whole ? last : ~0ull;
-  }
+  };
+  // by value alone: a key whose lower word tells the lanes apart and is left out of the bound
+  if (top && bounded) bound_warp(tid < (int)threads ? key_of(a.best, (uint32_t)tid) : 0);
   __syncthreads();
   {
     float m = -FLT_MAX;
@@ -335,37 +335,71 @@ __global__ void __launch_bounds__(THREADS) token_logprobs_kernel(const __grid_co
   // ---- the slice's largest
   if (top) {
     bool slow = all.s != all.s;          // a NaN or +inf: the maxima above passed over it
-    if (!slow) {
-      const bool bounded = threads >= top;
-      uint64_t bound = bounded ? sh[0] : 0;
-      if (bounded) {
+    const auto bound_of = [&]() {
+      uint64_t bound = sh[0];
 #pragma unroll
-        for (int w = 1; w < WARPS; ++w) bound = sh[w] < bound ? sh[w] : bound;
-      }
+      for (int w = 1; w < WARPS; ++w) bound = sh[w] < bound ? sh[w] : bound;
+      return bound;
+    };
+    const auto collect = [&](uint32_t u, uint64_t bound) {   // a piece's values that reach the bound
+      float x[N];
+      Vec<T>::widen(sl.piece(u), x);
       const float reach = value_of(bound);
-      // the threads that reach it (all that hold a piece, where there are fewer than `top` of those)
-      if (tid < (int)threads && mine >= bound) owners[atomicAdd(&owner_count, 1u)] = (uint16_t)tid;
-      __syncthreads();
-      const uint32_t each = (sl.pieces + THREADS - 1) / THREADS, n = owner_count * each;
-      for (uint32_t i = tid; i < n; i += THREADS) {
-        const uint32_t u = owners[i / each] + i % each * THREADS;
-        if (u < sl.pieces) {
-          const uint4 w = sl.piece(u);
-          if (bounded && Vec<T>::top(w) < reach) continue;   // nearly all
-          float x[N];
-          Vec<T>::widen(w, x);
 #pragma unroll
-          for (int e = 0; e < N; ++e) {
-            const int64_t col = sl.origin + (int64_t)u * N + e;
-            const uint64_t key = key_of(x[e], (uint32_t)col);
-            if (key >= bound && col >= sl.first && col < sl.last) {
-              const uint32_t k = atomicAdd(&count, 1u);
-              if (k < (uint32_t)HELD) held[k] = key;
-            }
+      for (int e = 0; e < N; ++e)
+        if (x[e] >= reach) {
+          const int64_t col = sl.origin + (int64_t)u * N + e;
+          const uint64_t key = key_of(x[e], (uint32_t)col);
+          if (key >= bound && col >= sl.first && col < sl.last) {
+            const uint32_t at = atomicAdd(&count, 1u);
+            if (at < (uint32_t)HELD) held[at] = key;
           }
+        }
+    };
+    const auto collect_owned = [&](uint64_t bound) {         // all pieces of the listed threads but the one each has done
+      const uint32_t rounds = (sl.pieces + THREADS - 1) / THREADS;
+      for (uint32_t o = warp; o < owner_count; o += WARPS)
+        for (uint32_t k = lane; k < rounds; k += 32) {
+          const uint32_t u = owners[o] + k * THREADS;
+          if (u < sl.pieces && u != done[o]) collect(u, bound);
+        }
+    };
+    const auto collect_all = [&](uint64_t bound, bool reaches, bool others) {
+      if (tid < (int)threads && reaches) {
+        collect(a.piece, bound);
+        if (others) {
+          const uint32_t at = atomicAdd(&owner_count, 1u);
+          owners[at] = (uint16_t)tid;
+          done[at] = a.piece;
         }
       }
       __syncthreads();
+      collect_owned(bound);
+      __syncthreads();
+    };
+    if (!slow) {
+      uint64_t bound = bounded ? bound_of() & 0xffffffff00000000ull : 0;
+      collect_all(bound, a.best >= value_of(bound), a.second >= value_of(bound));
+      if (count > (uint32_t)HELD && bounded) {
+        uint64_t mine = 0;               // this thread's largest key
+        if (tid < (int)threads) {
+          float x[N];
+          Vec<T>::widen(sl.piece(a.piece), x);
+          int at = -1;
+#pragma unroll
+          for (int e = N - 1; e >= 0; --e) {
+            const int64_t col = sl.origin + (int64_t)a.piece * N + e;
+            if (x[e] == a.best && col >= sl.first && col < sl.last) at = e;
+          }
+          if (at >= 0) mine = key_of(a.best, (uint32_t)(sl.origin + (int64_t)a.piece * N + at));
+        }
+        __syncthreads();                 // everyone has seen the count
+        if (tid == 0) count = owner_count = 0;
+        bound_warp(mine);
+        __syncthreads();
+        bound = bound_of();
+        collect_all(bound, mine >= bound, a.second >= value_of(bound));
+      }
       slow = count > (uint32_t)HELD;
       // the list's order depends on the atomics, its keys do not
       if (!slow)
@@ -449,16 +483,13 @@ __global__ void __launch_bounds__(THREADS) token_logprobs_kernel(const __grid_co
   if (tid == 0) {
     g.lse[r] = ref + log_sum;
     g.entropy[r] = entropy;
-    const int32_t id = g.ids[r];
-    float lp = 0.f;
-    if (id < -1 || (id >= 0 && id >= cols)) atomicCAS(g.err, 0, DOMAIN_ERROR);
-    else if (id >= 0) lp = log_prob(Vec<T>::one(row + id));
-    g.logprob[r] = lp;
+    if (!named && id != -1) atomicCAS(g.err, 0, DOMAIN_ERROR);
+    g.logprob[r] = named ? log_prob(id_logit) : 0.f;
   }
   if (warp == 0 && lane < (int)top) {
     const uint32_t col = col_of(list[lane]);
     g.top_ids[r * top + lane] = (int32_t)col;
-    g.top_logprobs[r * top + lane] = (int64_t)col < cols ? log_prob(Vec<T>::one(row + col)) : -INFINITY;
+    g.top_logprobs[r * top + lane] = log_prob(value_of(list[lane]));
   }
 }
 
