@@ -105,8 +105,9 @@ __device__ __forceinline__ void mma_tf32(float* c, uint32_t a0, uint32_t a1, uin
   asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// A value's leading TF32 part, cut, and what is left of it: exact, and a TF32 value but for its last two bits.
-__device__ __forceinline__ uint32_t tf32_of(float x) { return __float_as_uint(x) & 0xffffe000u; }
+// A value's leading TF32 part, to nearest, and what is left of it: exact, and a TF32 value but for its last bit.  (Cut, the left
+// would lose two bits, all toward zero: 7.6e-7 of a result in place of 5e-7.)
+__device__ __forceinline__ uint32_t tf32_of(float x) { return (__float_as_uint(x) + 0x1000u) & 0xffffe000u; }
 __device__ __forceinline__ uint32_t tf32_rest(float x) { return __float_as_uint(x - __uint_as_float(tf32_of(x))); }
 __device__ __forceinline__ float exp2_fast(float x) {   // the hardware's 2^x: 2 units in the last place, 2^-inf = 0
   float r;
@@ -406,11 +407,19 @@ __global__ void __launch_bounds__(Form<KV, D>::THREADS, Form<KV, D>::BLOCKS) att
         issue_keys();
 
         // running softmax: new maximum, the factor of what was summed before, the weights
+        const uint32_t off = live == 0xffffu ? 0u : ~live >> (2 * t4);         // bit 8 nt + e: not attended
+        float y[2][2];
 #pragma unroll
         for (int nt = 0; nt < 2; ++nt)
 #pragma unroll
-          for (int e = 0; e < 2; ++e) x[nt][e] = (live >> (nt * 8 + 2 * t4 + e)) & 1 ? x[nt][e] * a.scale_log2 : -INFINITY;
-        float top = fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[1][0], x[1][1]));
+          for (int e = 0; e < 2; ++e) y[nt][e] = x[nt][e] * a.scale_log2;
+        if (off) {
+#pragma unroll
+          for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) y[nt][e] = (off >> (8 * nt + e)) & 1 ? -INFINITY : y[nt][e];
+        }
+        float top = fmaxf(fmaxf(y[0][0], y[0][1]), fmaxf(y[1][0], y[1][1]));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
         top = fmaxf(top, m);
@@ -419,7 +428,13 @@ __global__ void __launch_bounds__(Form<KV, D>::THREADS, Form<KV, D>::BLOCKS) att
 #pragma unroll
         for (int nt = 0; nt < 2; ++nt)
 #pragma unroll
-          for (int e = 0; e < 2; ++e) x[nt][e] = exp2_fast(x[nt][e] - m);
+          for (int e = 0; e < 2; ++e) x[nt][e] = exp2_fast(fmaf(x[nt][e], a.scale_log2, -m));   // one rounding, of the difference
+        if (off) {
+#pragma unroll
+          for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) x[nt][e] = (off >> (8 * nt + e)) & 1 ? 0.f : x[nt][e];
+        }
         l = fmaf(l, f, (x[0][0] + x[0][1]) + (x[1][0] + x[1][1]));
 
         // rows = rows * factor + weights x values

@@ -493,10 +493,13 @@ __global__ void __launch_bounds__(THREADS) token_logprobs_kernel(const __grid_co
   }
 }
 
-// scale (g (1[j = id] - p) - h p (y - lse + H)) with p = e^(y - lse).  Both types are read and written in groups of eight
-// elements of the whole matrix, whose ends are the result's 16-byte boundaries whatever the row's length; a group that two rows
-// share is written by both, an element at a time.  A block takes SEGMENT groups a thread of one row.
-constexpr int SEGMENT = 8;
+// scale (g (1[j = id] - p) - h p (y - lse + H)) with p = e^(y - lse).  Memory-bound.  Both types are read and written in groups of
+// eight elements that start at the result's 16-byte boundaries whatever the row's length; a row's up to seven elements before its
+// first such group and behind its last are a thread each.
+// What a thread has in flight and how often: registers cost more here than bytes in flight bring (4000 x 32001 BF16: one group
+// four times 86 us, two groups four times 84, two once 87, four once 102 on fewer warps; 500 x 49152 F32, twice the bytes a group:
+// one once 30.6 us, two once 31.3, two four times 34.2).
+template <bool BF> struct Flight { static constexpr int GROUPS = BF ? 2 : 1, STEPS = BF ? 4 : 1; };
 // A group's values, and the LOW of the sums above in place of -inf: 0 times its exponent is 0.
 template <bool BF, bool ENTROPY>
 __device__ __forceinline__ void load_group(const LogprobGradArgs& g, uint64_t at, int vec, uint64_t* v) {
@@ -529,95 +532,71 @@ __device__ __forceinline__ void load_group(const LogprobGradArgs& g, uint64_t at
 }
 template <bool BF, bool OUT_BF, bool ENTROPY>
 __global__ void __launch_bounds__(256) token_logprobs_backward_kernel(const __grid_constant__ LogprobGradArgs g, uint32_t segments, int vec) {
-  constexpr int AHEAD = BF ? 4 : 2;      // groups asked for before the first is used: 64 bytes a thread
   pdl_enter();
-  const uint64_t r = blockIdx.x / segments, base = r * g.cols, end = base + g.cols;
-  const uint64_t first = base / 8 + (uint64_t)(blockIdx.x % segments) * SEGMENT * blockDim.x + threadIdx.x;
+  const uint32_t r = blockIdx.x / segments, segment = blockIdx.x % segments, cols = (uint32_t)g.cols;
+  const uint64_t base = (uint64_t)r * cols;
+  const uint32_t head = (uint32_t)(8 - (base & 7)) & 7, start = head < cols ? head : cols, groups = (cols - start) / 8;
+  uint32_t q = segment * (Flight<BF>::GROUPS * Flight<BF>::STEPS) * blockDim.x + threadIdx.x;
+  uint64_t x[Flight<BF>::GROUPS][4];
+#pragma unroll
+  for (int i = 0; i < Flight<BF>::GROUPS; ++i)
+    if (q + i * blockDim.x < groups) load_group<BF, ENTROPY>(g, base + start + (uint64_t)(q + i * blockDim.x) * 8, vec, x[i]);
   const float lse = g.lse[r], h = ENTROPY ? -g.d_entropy[r] * g.scale : 0.f, H = ENTROPY ? g.entropy[r] : 0.f;
-  int64_t id = g.ids[r];
-  if (id < -1 || id >= (int64_t)g.cols) {
-    if (threadIdx.x == 0) atomicCAS(g.err, 0, DOMAIN_ERROR);
-    id = -1;
-  }
-  const float up = id >= 0 ? g.d_logprob[r] * g.scale : 0.f;
-  const uint64_t hot = id >= 0 ? base + (uint64_t)id : ~0ull;
+  const float given = g.d_logprob[r] * g.scale;
+  const int32_t id = g.ids[r];
+  const bool named = id >= 0 && (uint32_t)id < cols;
+  if (!named && id != -1 && threadIdx.x == 0) atomicCAS(g.err, 0, DOMAIN_ERROR);
+  const float up = named ? given : 0.f;
+  const uint32_t hot = named ? (uint32_t)id : 0xffffffffu;
   const bool empty = lse == -INFINITY;
-  const uint64_t scale2 = pair_of(g.scale, g.scale), lse2 = pair_of(-lse, -lse), log2e2 = pair_of(LOG2E, LOG2E);
-  const uint64_t h2 = pair_of(h, h), base2 = ENTROPY ? pair_of(fmaf(h, H, -up), fmaf(h, H, -up)) : pair_of(-up, -up);
+  const float flat = ENTROPY ? fmaf(h, H, -up) : -up;
   // p (h (z + H) - up), z = y - lse
-  const auto value = [&](uint64_t x, float& v0, float& v1) {
-    const uint64_t z = fma2(x, scale2, lse2);
-    const float2 e = floats_of(mul2(z, log2e2));
-    const float2 k = floats_of(ENTROPY ? fma2(z, h2, base2) : base2);
+  const auto value = [&](uint64_t v, float& v0, float& v1) {
+    const uint64_t z = fma2(v, pair_of(g.scale, g.scale), pair_of(-lse, -lse));
+    const float2 e = floats_of(mul2(z, pair_of(LOG2E, LOG2E)));
+    const float2 k = floats_of(ENTROPY ? fma2(z, pair_of(h, h), pair_of(flat, flat)) : pair_of(flat, flat));
     v0 = mul_flush(exp2_fast(e.x), k.x);
     v1 = mul_flush(exp2_fast(e.y), k.y);
   };
-  const auto patch = [&](uint64_t at, float (&v)[8]) {       // the given token's own term, and a row of -inf only
-    if (hot - at < 8)
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (at + e == hot) v[e] += up;
-    if (empty)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = 0.f;
-  };
-  const auto put = [&](uint64_t at, const float (&v)[8]) {
-    if constexpr (OUT_BF) {
-      uint32_t w[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w[e]) : "f"(v[2 * e + 1]), "f"(v[2 * e]));
-      *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(g.out) + at) = make_uint4(w[0], w[1], w[2], w[3]);
-    } else {
-      float4* o = reinterpret_cast<float4*>(reinterpret_cast<float*>(g.out) + at);
-      o[0] = make_float4(v[0], v[1], v[2], v[3]);
-      o[1] = make_float4(v[4], v[5], v[6], v[7]);
-    }
-  };
-  // the block's groups; all of them inside the row but for its first and last segment
-  const uint64_t begin = first - threadIdx.x, stop = begin + (uint64_t)SEGMENT * blockDim.x;
-  const bool inner = begin * 8 >= base && stop * 8 <= end;
-  const bool plain = !empty && (hot < begin * 8 || hot >= stop * 8);
 #pragma unroll 1
-  for (int step = 0; step < SEGMENT; step += AHEAD) {
-    const uint64_t at0 = (first + (uint64_t)step * blockDim.x) * 8, apart = (uint64_t)blockDim.x * 8;
-    if (inner) {
-      uint64_t x[AHEAD][4];
+  for (int step = 0;; ++step) {
 #pragma unroll
-      for (int i = 0; i < AHEAD; ++i) load_group<BF, ENTROPY>(g, at0 + i * apart, vec, x[i]);
+    for (int i = 0; i < Flight<BF>::GROUPS; ++i) {
+      const uint32_t at = q + i * blockDim.x, col = start + at * 8;
+      if (at >= groups) break;
+      float v[8];
 #pragma unroll
-      for (int i = 0; i < AHEAD; ++i) {
-        float v[8];
+      for (int e = 0; e < 4; ++e) value(x[i][e], v[2 * e], v[2 * e + 1]);
+      if (hot - col < 8 || empty)                            // the given token's own term, and a row of -inf only
 #pragma unroll
-        for (int e = 0; e < 4; ++e) value(x[i][e], v[2 * e], v[2 * e + 1]);
-        if (!plain) patch(at0 + i * apart, v);
-        put(at0 + i * apart, v);
+        for (int e = 0; e < 8; ++e) v[e] = empty ? 0.f : (col + e == hot ? v[e] + up : v[e]);
+      if constexpr (OUT_BF) {
+        uint32_t w[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w[e]) : "f"(v[2 * e + 1]), "f"(v[2 * e]));
+        *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(g.out) + base + col) = make_uint4(w[0], w[1], w[2], w[3]);
+      } else {
+        float4* o = reinterpret_cast<float4*>(reinterpret_cast<float*>(g.out) + base + col);
+        o[0] = make_float4(v[0], v[1], v[2], v[3]);
+        o[1] = make_float4(v[4], v[5], v[6], v[7]);
       }
-      continue;
     }
-    for (int i = 0; i < AHEAD; ++i) {
-      const uint64_t at = at0 + i * apart;
-      if (at >= end) break;
-      if (at >= base && at + 8 <= end) {
-        uint64_t x[4];
-        load_group<BF, ENTROPY>(g, at, vec, x);
-        float v[8];
+    q += Flight<BF>::GROUPS * blockDim.x;
+    if (step + 1 == Flight<BF>::STEPS || q >= groups) break;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) value(x[e], v[2 * e], v[2 * e + 1]);
-        patch(at, v);
-        put(at, v);
-      } else {                                               // a group that this row shares with another
-        for (int e = 0; e < 8; ++e) {
-          if (at + e < base || at + e >= end) continue;
-          float y = BF ? bf16_bits_to_f32(reinterpret_cast<const uint16_t*>(g.logits)[at + e]) : reinterpret_cast<const float*>(g.logits)[at + e];
-          if (y < LOW) y = LOW;
-          float v, other;
-          value(pair_of(y, y), v, other);
-          if (at + e == hot) v += up;
-          if (empty) v = 0.f;
-          if constexpr (OUT_BF) reinterpret_cast<uint16_t*>(g.out)[at + e] = f32_to_bf16_bits(__float_as_uint(v));
-          else reinterpret_cast<float*>(g.out)[at + e] = v;
-        }
-      }
+    for (int i = 0; i < Flight<BF>::GROUPS; ++i)
+      if (q + i * blockDim.x < groups) load_group<BF, ENTROPY>(g, base + start + (uint64_t)(q + i * blockDim.x) * 8, vec, x[i]);
+  }
+  if (segment == 0 && threadIdx.x < 16) {
+    const uint32_t end = start + groups * 8, col = threadIdx.x < 8 ? threadIdx.x : end + threadIdx.x - 8;
+    if (threadIdx.x < 8 ? col < start : col < cols) {
+      const float y = BF ? bf16_bits_to_f32(reinterpret_cast<const uint16_t*>(g.logits)[base + col]) : reinterpret_cast<const float*>(g.logits)[base + col];
+      const float z = y < LOW ? LOW : y;
+      float v, other;
+      value(pair_of(z, z), v, other);
+      v = empty ? 0.f : (col == hot ? v + up : v);
+      if constexpr (OUT_BF) reinterpret_cast<uint16_t*>(g.out)[base + col] = f32_to_bf16_bits(__float_as_uint(v));
+      else reinterpret_cast<float*>(g.out)[base + col] = v;
     }
   }
 }
@@ -658,10 +637,10 @@ cudaError_t launch_token_logprobs(const LogprobArgs& g, cudaStream_t stream) {
 
 cudaError_t launch_token_logprobs_backward(const LogprobGradArgs& g, cudaStream_t stream) {
   if (g.rows == 0) return cudaSuccess;
-  const uint64_t groups = (g.cols + 7) / 8 + 1;            // a row that starts inside a group touches one more
+  const uint64_t groups = g.cols / 8, each = g.bf16 ? Flight<true>::GROUPS * Flight<true>::STEPS : Flight<false>::GROUPS * Flight<false>::STEPS;
   unsigned threads = 32;
-  while (threads < 256 && threads * SEGMENT < groups) threads *= 2;
-  const uint64_t segments = (groups + threads * SEGMENT - 1) / (threads * SEGMENT), blocks = segments * g.rows;
+  while (threads < 256 && threads * each < groups) threads *= 2;
+  const uint64_t segments = groups ? (groups + threads * each - 1) / (threads * each) : 1, blocks = segments * g.rows;
   if (blocks > 0x7fffffffull) return cudaErrorNotSupported;
   const int vec = (reinterpret_cast<uintptr_t>(g.logits) & 15) == 0;
   const auto go = [&](auto kernel) { launch_pdl(kernel, dim3((unsigned)blocks), dim3(threads), 0, stream, g, (uint32_t)segments, vec); };
