@@ -621,11 +621,17 @@ cudaError_t launch_form(const LogprobArgs& g, int size, cudaStream_t stream) {
 
 template <typename T>
 cudaError_t launch_type(const LogprobArgs& g, cudaStream_t stream) {
-  // A row's blocks: as many as leave every block a slice of some thousand values while the rows alone do not fill the GPU.
+  // A row's blocks: as many as leave every block a slice of some thousand values while the rows alone do not fill the GPU (one F32
+  // row of 49,152 with five alternatives: 8.7 us by a cluster of eight, 16.1 by one block; of 260,000 with twenty: 16 and 65).
   int size = 1;
   while (size < CLUSTER && g.rows * size < 296 && g.cols / (size * 2) >= 2048) size *= 2;
   if (size > 1) return launch_form<T, 256, true>(g, size, stream);
-  return g.cols <= 1024 ? launch_form<T, 32, false>(g, 1, stream) : launch_form<T, 256, false>(g, 1, stream);
+  // A row's threads: what a row's end costs grows with its block, what a thread has in flight is the same, so blocks are small as
+  // long as there are enough of them to fill the GPU.  64 MB of BF16 logits with twenty alternatives by 32 / 64 / 128 / 256
+  // threads a row, us: rows of 2,000 67 / 64 / 83 / 137, of 4,000 46 / 41 / 50 / 84, of 8,000 35 / 31 / 33 / 50, of 16,000
+  // 49 / 30 / 27 / 33, of 32,000 70 / 35 / 26 / 28; 4,000 rows of 1,000 9 / - / - / 28.
+  if (g.cols <= 1024) return launch_form<T, 32, false>(g, 1, stream);
+  return g.cols <= 10000 ? launch_form<T, 64, false>(g, 1, stream) : launch_form<T, 128, false>(g, 1, stream);
 }
 
 }  // namespace
