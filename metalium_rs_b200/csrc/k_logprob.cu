@@ -342,9 +342,11 @@ __global__ void __launch_bounds__(THREADS) token_logprobs_kernel(const __grid_co
       return bound;
     };
     const auto collect = [&](uint32_t u, uint64_t bound) {   // a piece's values that reach the bound
-      float x[N];
-      Vec<T>::widen(sl.piece(u), x);
+      const uint4 w = sl.piece(u);
       const float reach = value_of(bound);
+      if (Vec<T>::top(w) < reach) return;
+      float x[N];
+      Vec<T>::widen(w, x);
 #pragma unroll
       for (int e = 0; e < N; ++e)
         if (x[e] >= reach) {
@@ -357,12 +359,11 @@ __global__ void __launch_bounds__(THREADS) token_logprobs_kernel(const __grid_co
         }
     };
     const auto collect_owned = [&](uint64_t bound) {         // all pieces of the listed threads but the one each has done
-      const uint32_t rounds = (sl.pieces + THREADS - 1) / THREADS;
-      for (uint32_t o = warp; o < owner_count; o += WARPS)
-        for (uint32_t k = lane; k < rounds; k += 32) {
-          const uint32_t u = owners[o] + k * THREADS;
-          if (u < sl.pieces && u != done[o]) collect(u, bound);
-        }
+      const uint32_t rounds = (sl.pieces + THREADS - 1) / THREADS, n = owner_count * rounds;
+      for (uint32_t i = tid; i < n; i += THREADS) {
+        const uint32_t o = i / rounds, u = owners[o] + i % rounds * THREADS;
+        if (u < sl.pieces && u != done[o]) collect(u, bound);
+      }
     };
     const auto collect_all = [&](uint64_t bound, bool reaches, bool others) {
       if (tid < (int)threads && reaches) {
