@@ -242,9 +242,15 @@ __device__ __forceinline__ uint32_t place_of(uint64_t key, const uint64_t* keys,
 // piece of its largest again, and only where another of its pieces reaches it too (one thread in ten of those) are all of that
 // thread's read by the block.  What reaches the bound is listed and put in order.  Where that is more than the list holds -- rows
 // of few distinct values -- the bound is taken again from keys, by value and column.
+//
+// A thread asks for AHEAD of its pieces before it uses the first.  Eight where rows are long, with six blocks a SM: without
+// alternatives 2000 BF16 rows of 50257 take 42.6 us (4.7 TB/s) for 44.8 with four, 1000 F32 rows 34.9 (5.8 TB/s) for 39.2; seven
+// blocks a SM leave too few registers (46.8 and 37.3).  Four in the other forms, whose threads have few pieces, and as many
+// blocks as the registers allow (0): more of either costs 16000 rows of 2000 59 -> 70 us and above.
+// Bound by the instructions issued, not by memory: two exponents' and five pairs' operations a pair of values.
 template <typename T, int THREADS, bool SHARED>
-__global__ void __launch_bounds__(THREADS) token_logprobs_kernel(const __grid_constant__ LogprobArgs g) {
-  constexpr int WARPS = THREADS / 32, N = Vec<T>::N, HELD = THREADS * 8;
+__global__ void __launch_bounds__(THREADS, THREADS == 128 ? 6 : 0) token_logprobs_kernel(const __grid_constant__ LogprobArgs g) {
+  constexpr int WARPS = THREADS / 32, N = Vec<T>::N, HELD = THREADS * 8, AHEAD = THREADS == 128 ? 8 : 4;
   __shared__ uint64_t held[HELD], sh[WARPS], slices[SHARED ? CLUSTER * TOP : TOP], list[TOP];
   __shared__ Sums warp_sums[WARPS], slice_sums[SHARED ? CLUSTER : 1];
   __shared__ float warp_best[WARPS], slice_best[SHARED ? CLUSTER : 1];
@@ -272,18 +278,18 @@ __global__ void __launch_bounds__(THREADS) token_logprobs_kernel(const __grid_co
   const bool named = id >= 0 && id < cols;
   const float id_logit = named ? Vec<T>::one(row + id) : 0.f;
 
-  // ---- the pass: four pieces of a thread asked for before the first is used; the slice's cut ends by themselves
+  // ---- the pass; the slice's cut ends by themselves
   Running<T> a;
   a.piece = (uint32_t)tid;               // a thread whose values are all -inf has its first
   const uint32_t lo = sl.pieces && !sl.whole(0) ? 1u : 0u, hi = sl.pieces && !sl.whole(sl.pieces - 1) ? sl.pieces - 1 : sl.pieces;
   if (lo && tid == 0) a.take(sl.piece(0), 0, c, c2);
-  for (uint32_t u = lo && tid == 0 ? THREADS : tid; u < hi; u += 4 * THREADS) {
-    uint4 w[4];
+  for (uint32_t u = lo && tid == 0 ? THREADS : tid; u < hi; u += AHEAD * THREADS) {
+    uint4 w[AHEAD];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < AHEAD; ++i)
       if (u + i * THREADS < hi) w[i] = sl.raw(u + i * THREADS);
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < AHEAD; ++i)
       if (u + i * THREADS < hi) a.take(w[i], u + i * THREADS, c, c2);
   }
   if (hi < sl.pieces && hi >= lo && sl.pieces > lo && tid == (int)(hi % THREADS)) a.take(sl.piece(hi), hi, c, c2);
@@ -630,7 +636,7 @@ cudaError_t launch_type(const LogprobArgs& g, cudaStream_t stream) {
   // A row's threads: what a row's end costs grows with its block, what a thread has in flight is the same, so blocks are small as
   // long as there are enough of them to fill the GPU.  64 MB of BF16 logits with twenty alternatives by 32 / 64 / 128 / 256
   // threads a row, us: rows of 2,000 67 / 64 / 83 / 137, of 4,000 46 / 41 / 50 / 84, of 8,000 35 / 31 / 33 / 50, of 16,000
-  // 49 / 30 / 27 / 33, of 32,000 70 / 35 / 26 / 28; 4,000 rows of 1,000 9 / - / - / 28.
+  // 49 / 30 / 26 / 33, of 32,000 70 / 35 / 22 / 28; 4,000 rows of 1,000 9 / - / - / 28.
   if (g.cols <= 1024) return launch_form<T, 32, false>(g, 1, stream);
   return g.cols <= 10000 ? launch_form<T, 64, false>(g, 1, stream) : launch_form<T, 128, false>(g, 1, stream);
 }

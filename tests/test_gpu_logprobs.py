@@ -109,6 +109,23 @@ def test_logprobs_of_any_count_of_rows(eng, rows, cols):
 
 
 @pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("rows,cols", [(300, 1500), (297, 9999), (296, 10001), (310, 20011), (296, 33000)])
+def test_many_rows_with_hard_ones_among_them(eng, rows, cols, bf16):
+    # Rows enough to fill the GPU one a block: every eighth is of few values, masked, rising or holds a NaN or an infinity.
+    rng = np.random.default_rng(cols)
+    x = logits(rng, rows, cols)
+    hard = [np.full(cols, -2.5), np.full(cols, -np.inf), np.where(np.arange(cols) == cols - 1, 1.0, -np.inf),
+            np.arange(cols) // (cols // 200), np.arange(cols)[::-1] // (cols // 200), rng.integers(-1, 2, cols),
+            np.where(np.arange(cols) == cols // 2, np.nan, 0.5), np.where(np.arange(cols) == 1, np.inf, 0.5),
+            np.where(rng.random(cols) < 0.999, -3.0e38, 4.0), np.where(np.arange(cols) < cols - 7, -np.inf, 2.0)]
+    for i in range(0, rows, 8):
+        x[i] = hard[i // 8 % len(hard)]
+    ids = rng.integers(-1, cols, rows)
+    for top, view in ((20, 0), (32, 3), (0, 1)):
+        check(eng, x, ids, 0.9, top, bf16, view)
+
+
+@pytest.mark.parametrize("bf16", [False, True])
 @pytest.mark.parametrize("cols", [33, 1000, 5000, 49153])
 def test_equal_values_go_by_the_lower_column(eng, cols, bf16):
     rng = np.random.default_rng(cols)
