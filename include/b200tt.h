@@ -456,9 +456,9 @@ int32_t b200_decode_layers(b200_engine*, const b200_decode_shape* shape, b200_bu
  *   positions               I32, one value a row of the call; -1 marks a padding row or an idle slot.
  * A position behind the table's last page (or, with a rotation, outside the cos and sin tables) or below -1, a sequence outside
  * the table or a page number outside the pool sets DOMAIN on the device: the row is then treated as padding (in attention, a
- * page outside the pool is left out and the others attended), and nothing outside the buffers is touched.  `into` is 0 or a live buffer of the result's dims and element type at a
- * 16-byte address that shares no memory with the call's other buffers: the result is then written there (and *out = into)
- * instead of into a new buffer. */
+ * page outside the pool is left out and the others attended), and nothing outside the buffers is touched.  `into` is 0 or a
+ * live buffer of the result's dims and element type at a 16-byte address that shares no memory with the call's other buffers:
+ * the result is then written there (and *out = into) instead of into a new buffer. */
 typedef struct { uint32_t heads, kv_heads, head_dim, page_size; } b200_page_shape;
 /* The rotation of `rope_blocks` (server.rs:566) on a projection's query and key heads and the cache write of
  * `scatter_rows_into` (server.rs:389) as one pass: qkv is a block [n, (heads + 2 kv_heads) head_dim] (Wq | Wk | Wv side by
@@ -479,8 +479,10 @@ int32_t b200_rope_append_pages(b200_engine*, const b200_page_shape* shape, const
  * the cache already; query head h reads key/value head h / (heads / kv_heads).  It attends to positions 0 .. positions[i], or
  * with window > 0 to the last `window` of them.  out [n, heads * head_dim] = softmax(scale q K^T) V with `attention_rows`'
  * steps in F32 (clamped maximum and sum: a row that attends to nothing, positions[i] == -1 or scores all -inf, is zero),
- * rounded once with out_bf16.  Nothing behind a sequence's last position is read.  Refused unless head_dim is 32, 64, 96,
- * 128, 192 or 256 and heads is a multiple of kv_heads. */
+ * rounded once with out_bf16.  Nothing behind a sequence's last position is read.  An infinite or NaN value at an attended
+ * position makes its column NaN (infinite keys give what their scores are); F32 values are below 3.4e38 in magnitude.
+ * Refused unless head_dim is 32, 64, 96, 128, 192 or 256, heads is a multiple of kv_heads and scale lies within
+ * -1e20 .. 1e20. */
 int32_t b200_attention_pages(b200_engine*, const b200_page_shape* shape, const b200_block_arg* q, b200_buffer key_pages,
                              b200_buffer value_pages, b200_buffer page_table, b200_buffer positions, uint32_t window, float scale,
                              int32_t out_bf16, b200_buffer into, b200_buffer* out, uint64_t out_dims[2]);
@@ -495,14 +497,15 @@ int32_t b200_attention_pages(b200_engine*, const b200_page_shape* shape, const b
  * One pass over the logits; sums in F32 under the row's maximum.  A row of -inf only has lse -inf, entropy 0 and log
  * probabilities -inf; a row with a NaN or +inf has NaN in all three.  Another id outside the columns sets DOMAIN (and gives 0).
  * `into` is NULL or five ids as `b200_rope_append_pages` takes one (0: a new buffer).  Refused unless scale lies
- * within 1e-20 .. 1e20, top <= 32 and top <= vocab. */
+ * within 1e-20 .. 1e6, top <= 32 and top <= vocab. */
 int32_t b200_token_logprobs(b200_engine*, b200_buffer logits, b200_buffer ids, float scale, uint32_t top, const b200_buffer into[5],
                             b200_buffer out[5], uint64_t out_dims[2]);
 /* The gradient of the first two with respect to the logits: with p = exp(y - lse) and the rows' upstream gradients
  * d_logprob and d_entropy (F32, rows values; d_entropy and entropy 0: absent),
  *   out = scale * (d_logprob (1[column = id] - p) - d_entropy p (y - lse + entropy)),
  * F32 or rounded once to BF16, [rows, vocab].  lse and entropy are the forward's.  A row whose id is -1 has no d_logprob
- * term; an entry of -inf has gradient 0 (its own 1[column = id] term apart), a row of -inf only is zero. */
+ * term; an entry of -inf has gradient 0 (its own 1[column = id] term apart), a row of -inf only is zero.  Refused as the
+ * forward is. */
 int32_t b200_token_logprobs_backward(b200_engine*, b200_buffer logits, b200_buffer ids, b200_buffer lse, b200_buffer entropy,
                                      b200_buffer d_logprob, b200_buffer d_entropy, float scale, int32_t out_bf16,
                                      b200_buffer into, b200_buffer* out, uint64_t out_dims[2]);

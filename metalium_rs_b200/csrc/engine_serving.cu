@@ -97,8 +97,8 @@ int page_view(b200_engine* e, const b200_page_shape* shape, b200_buffer key_page
   return B200_OK;
 }
 
-// Within what an F32 logit times it can be told from -inf by.
-bool good_scale(float s) { return s >= 1e-20f && s <= 1e20f; }
+// What stands for -inf in a row's sums, -1e30, times the scale and log2 e has to stay a finite number far below every term.
+bool good_scale(float s) { return s >= 1e-20f && s <= 1e6f; }
 
 // `rows` F32 values as one row or one column (a per-row statistic or gradient).
 int row_values(b200_engine* e, b200_buffer id, uint64_t rows, Buf** b, const char* name, const char* what) {
@@ -138,7 +138,7 @@ int32_t b200_rope_append_pages(b200_engine* e, const b200_page_shape* shape, con
   if (g.qkv.cols != ((uint64_t)shape->heads + 2ull * shape->kv_heads) * d)
     return e->fail(B200_UNSUPPORTED, "%s: %llu columns are not %u query and 2 x %u key and value heads of %u", what, (ull)g.qkv.cols, shape->heads,
                    shape->kv_heads, shape->head_dim);
-  if (n > 0x7fffffffull) return e->fail(B200_UNSUPPORTED, "%s: %llu rows", what, (ull)n);
+  if (n > 0x7fffffffull || g.qkv.cols > 0x7fffffffull) return e->fail(B200_UNSUPPORTED, "%s: [%llu, %llu] rows", what, (ull)n, (ull)g.qkv.cols);
   st = int_list(e, positions, n, &P, "positions", what);
   if (!st && sequences) st = int_list(e, sequences, n, &S, "sequences", what);
   if (st) return st;
@@ -189,7 +189,7 @@ int32_t b200_attention_pages(b200_engine* e, const b200_page_shape* shape, const
   if (!attention_pages_dim_ok(shape->head_dim)) return e->fail(B200_UNSUPPORTED, "%s: heads of %u columns (32, 64, 96, 128, 192 or 256)", what, shape->head_dim);
   if (g.q.cols != cols) return e->fail(B200_UNSUPPORTED, "%s: %llu query columns for %u heads of %u", what, (ull)g.q.cols, shape->heads, shape->head_dim);
   if (n > g.cache.sequences) return e->fail(B200_UNSUPPORTED, "%s: %llu rows and a page table of %u sequences", what, (ull)n, g.cache.sequences);
-  if (!std::isfinite(scale)) return e->fail(B200_UNSUPPORTED, "%s: the scale is not finite", what);
+  if (!(std::fabs(scale) <= 1e20f)) return e->fail(B200_UNSUPPORTED, "%s: the scale %g is not within -1e20 .. 1e20", what, scale);
   st = int_list(e, positions, n, &P, "positions", what);
   if (st) return st;
   spans.push_back(span_of(Q)); spans.push_back(span_of(P));
@@ -222,7 +222,7 @@ int32_t b200_token_logprobs(b200_engine* e, b200_buffer logits, b200_buffer ids,
   const uint64_t rows = X->rows, cols = X->cols;
   st = int_list(e, ids, rows, &I, "ids", what);
   if (st) return st;
-  if (!good_scale(scale)) return e->fail(B200_UNSUPPORTED, "%s: the scale %g is not within 1e-20 .. 1e20", what, scale);
+  if (!good_scale(scale)) return e->fail(B200_UNSUPPORTED, "%s: the scale %g is not within 1e-20 .. 1e6", what, scale);
   if (top > 32 || top > cols) return e->fail(B200_UNSUPPORTED, "%s: the %u largest of %llu columns (at most 32)", what, top, (ull)cols);
   LogprobArgs g;
   g.logits = X->ptr; g.bf16 = X->elem == B200_BF16; g.rows = rows; g.cols = cols;
@@ -259,7 +259,7 @@ int32_t b200_token_logprobs_backward(b200_engine* e, b200_buffer logits, b200_bu
   if (!st && d_entropy) st = row_values(e, d_entropy, rows, &GH, "d_entropy", what);
   if (!st && d_entropy) st = row_values(e, entropy, rows, &H, "entropy", what);
   if (st) return st;
-  if (!good_scale(scale)) return e->fail(B200_UNSUPPORTED, "%s: the scale %g is not within 1e-20 .. 1e20", what, scale);
+  if (!good_scale(scale)) return e->fail(B200_UNSUPPORTED, "%s: the scale %g is not within 1e-20 .. 1e6", what, scale);
   std::vector<Span> spans = {span_of(X), span_of(I), span_of(L), span_of(G)};
   if (GH) { spans.push_back(span_of(GH)); spans.push_back(span_of(H)); }
   Result r;

@@ -33,6 +33,11 @@ __device__ __forceinline__ float mul_flush(float a, float b) {
   asm("mul.ftz.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
+__device__ __forceinline__ float at_least(float x, float low) {   // a NaN stays one
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(low));
+  return r;
+}
 // Two F32 operations an instruction.
 __device__ __forceinline__ uint64_t pair_of(float a, float b) {
   uint64_t r;
@@ -87,11 +92,7 @@ template <> struct Vec<float> {
   static __device__ __forceinline__ float top(const uint4& w) {
     return fmaxf(fmaxf(__uint_as_float(w.x), __uint_as_float(w.y)), fmaxf(__uint_as_float(w.z), __uint_as_float(w.w)));
   }
-  static __device__ __forceinline__ float low(uint32_t w) {
-    float r;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(__uint_as_float(w)), "f"(LOW));
-    return r;
-  }
+  static __device__ __forceinline__ float low(uint32_t w) { return at_least(__uint_as_float(w), LOW); }
   static __device__ __forceinline__ void pairs(const uint4& w, uint64_t* v) { v[0] = pair_of(low(w.x), low(w.y)); v[1] = pair_of(low(w.z), low(w.w)); }
 };
 template <> struct Vec<uint16_t> {
@@ -507,21 +508,15 @@ __global__ void __launch_bounds__(THREADS, THREADS == 128 ? 6 : 0) token_logprob
 // four times 86 us, two groups four times 84, two once 87, four once 102 on fewer warps; 500 x 49152 F32, twice the bytes a group:
 // one once 30.6 us, two once 31.3, two four times 34.2).
 template <bool BF> struct Flight { static constexpr int GROUPS = BF ? 2 : 1, STEPS = BF ? 4 : 1; };
-// A group's values, and the LOW of the sums above in place of -inf: 0 times its exponent is 0.
-template <bool BF, bool ENTROPY>
+template <bool BF>
 __device__ __forceinline__ void load_group(const LogprobGradArgs& g, uint64_t at, int vec, uint64_t* v) {
+  float x[8];
   if constexpr (BF) {
     const uint16_t* p = reinterpret_cast<const uint16_t*>(g.logits) + at;
     uint4 w;
     if (vec) w = __ldg(reinterpret_cast<const uint4*>(p));
     else w = make_uint4(p[0] | (uint32_t)p[1] << 16, p[2] | (uint32_t)p[3] << 16, p[4] | (uint32_t)p[5] << 16, p[6] | (uint32_t)p[7] << 16);
-    if constexpr (ENTROPY) Vec<uint16_t>::pairs(w, v);
-    else {
-      float x[8];
-      Vec<uint16_t>::widen(w, x);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = pair_of(x[2 * i], x[2 * i + 1]);
-    }
+    Vec<uint16_t>::widen(w, x);
   } else {
     const float* p = reinterpret_cast<const float*>(g.logits) + at;
     uint4 w[2];
@@ -530,12 +525,11 @@ __device__ __forceinline__ void load_group(const LogprobGradArgs& g, uint64_t at
       const uint32_t* q = reinterpret_cast<const uint32_t*>(p);
       w[0] = make_uint4(q[0], q[1], q[2], q[3]); w[1] = make_uint4(q[4], q[5], q[6], q[7]);
     }
-    if constexpr (ENTROPY) { Vec<float>::pairs(w[0], v); Vec<float>::pairs(w[1], v + 2); }
-    else {
-      v[0] = pair_of(__uint_as_float(w[0].x), __uint_as_float(w[0].y)); v[1] = pair_of(__uint_as_float(w[0].z), __uint_as_float(w[0].w));
-      v[2] = pair_of(__uint_as_float(w[1].x), __uint_as_float(w[1].y)); v[3] = pair_of(__uint_as_float(w[1].z), __uint_as_float(w[1].w));
-    }
+    Vec<float>::widen(w[0], x);
+    Vec<float>::widen(w[1], x + 4);
   }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = pair_of(x[2 * i], x[2 * i + 1]);
 }
 template <bool BF, bool OUT_BF, bool ENTROPY>
 __global__ void __launch_bounds__(256) token_logprobs_backward_kernel(const __grid_constant__ LogprobGradArgs g, uint32_t segments, int vec) {
@@ -547,7 +541,7 @@ __global__ void __launch_bounds__(256) token_logprobs_backward_kernel(const __gr
   uint64_t x[Flight<BF>::GROUPS][4];
 #pragma unroll
   for (int i = 0; i < Flight<BF>::GROUPS; ++i)
-    if (q + i * blockDim.x < groups) load_group<BF, ENTROPY>(g, base + start + (uint64_t)(q + i * blockDim.x) * 8, vec, x[i]);
+    if (q + i * blockDim.x < groups) load_group<BF>(g, base + start + (uint64_t)(q + i * blockDim.x) * 8, vec, x[i]);
   const float lse = g.lse[r], h = ENTROPY ? -g.d_entropy[r] * g.scale : 0.f, H = ENTROPY ? g.entropy[r] : 0.f;
   const float given = g.d_logprob[r] * g.scale;
   const int32_t id = g.ids[r];
@@ -557,9 +551,10 @@ __global__ void __launch_bounds__(256) token_logprobs_backward_kernel(const __gr
   const uint32_t hot = named ? (uint32_t)id : 0xffffffffu;
   const bool empty = lse == -INFINITY;
   const float flat = ENTROPY ? fmaf(h, H, -up) : -up;
-  // p (h (z + H) - up), z = y - lse
+  // p (h (z + H) - up), z = y - lse; with a z below -1000, where p is 0, its factor stays finite
   const auto value = [&](uint64_t v, float& v0, float& v1) {
-    const uint64_t z = fma2(v, pair_of(g.scale, g.scale), pair_of(-lse, -lse));
+    uint64_t z = fma2(v, pair_of(g.scale, g.scale), pair_of(-lse, -lse));
+    if constexpr (ENTROPY) z = pair_of(at_least(floats_of(z).x, -1000.f), at_least(floats_of(z).y, -1000.f));
     const float2 e = floats_of(mul2(z, pair_of(LOG2E, LOG2E)));
     const float2 k = floats_of(ENTROPY ? fma2(z, pair_of(h, h), pair_of(flat, flat)) : pair_of(flat, flat));
     v0 = mul_flush(exp2_fast(e.x), k.x);
@@ -592,15 +587,14 @@ __global__ void __launch_bounds__(256) token_logprobs_backward_kernel(const __gr
     if (step + 1 == Flight<BF>::STEPS || q >= groups) break;
 #pragma unroll
     for (int i = 0; i < Flight<BF>::GROUPS; ++i)
-      if (q + i * blockDim.x < groups) load_group<BF, ENTROPY>(g, base + start + (uint64_t)(q + i * blockDim.x) * 8, vec, x[i]);
+      if (q + i * blockDim.x < groups) load_group<BF>(g, base + start + (uint64_t)(q + i * blockDim.x) * 8, vec, x[i]);
   }
   if (segment == 0 && threadIdx.x < 16) {
     const uint32_t end = start + groups * 8, col = threadIdx.x < 8 ? threadIdx.x : end + threadIdx.x - 8;
     if (threadIdx.x < 8 ? col < start : col < cols) {
       const float y = BF ? bf16_bits_to_f32(reinterpret_cast<const uint16_t*>(g.logits)[base + col]) : reinterpret_cast<const float*>(g.logits)[base + col];
-      const float z = y < LOW ? LOW : y;
       float v, other;
-      value(pair_of(z, z), v, other);
+      value(pair_of(y, y), v, other);
       v = empty ? 0.f : (col == hot ? v + up : v);
       if constexpr (OUT_BF) reinterpret_cast<uint16_t*>(g.out)[base + col] = f32_to_bf16_bits(__float_as_uint(v));
       else reinterpret_cast<float*>(g.out)[base + col] = v;

@@ -180,6 +180,18 @@ def test_large_logits_keep_their_differences(eng):
     check(eng, x, np.array([5, 7, 2999]), 1.0, 5)
 
 
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("cols", [100, 3001, 50001])
+@pytest.mark.parametrize("scale", [1.0e-20, 1.0e-6, 1.0e6])
+def test_masked_logits_at_the_ends_of_the_scale(eng, cols, bf16, scale):
+    rng = np.random.default_rng(cols)
+    x = (logits(rng, 5, cols) / np.float32(scale)).astype(np.float32)    # 3e21 at most
+    x[:, rng.random(cols) < 0.5] = -np.inf
+    x[:, 0] = 0.0
+    x[1, 1:] = -np.inf
+    check(eng, x, np.array([0, 0, 0, -1, 0]), scale, 20, bf16)
+
+
 def test_a_token_outside_the_columns_is_reported(fresh_eng):
     e = fresh_eng
     x = np.zeros((3, 10), np.float32)
@@ -274,6 +286,22 @@ def test_gradient_of_masked_rows(eng, cols):
     assert np.isfinite(got).all() and not got[0].any()
     assert np.all(np.abs(got - want) <= tol)
     assert not got[np.isneginf(x) & (np.arange(cols)[None, :] != ids[:, None])].any()
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("scale,h", [(1.0, 1.0e10), (1.0, 1.0e30), (1.0e6, 1.0), (1.0e6, 1.0e6), (1.0e-20, 1.0)])
+def test_masked_entries_have_no_gradient_whatever_the_factors(eng, scale, h, bf16):
+    # 0 times an infinite factor would be NaN
+    rng = np.random.default_rng(17)
+    x = (logits(rng, 5, 1003) / np.float32(scale)).astype(np.float32)
+    x[:, rng.random(1003) < 0.5] = -np.inf
+    x[:, [0, 500, 1002]] = 0.0
+    x[2, 500] = -3.0e38
+    ids = np.array([0, 500, 1002, -1, 0])
+    got, want, tol = backward(eng, x, ids, rng.standard_normal(5), np.full(5, h), scale, bf16, False)
+    assert np.isfinite(got).all()
+    assert not got[np.isneginf(x)].any()
+    assert np.all(np.abs(got - want) <= tol)
 
 
 def test_gradient_against_differences(eng):

@@ -203,6 +203,25 @@ def test_logprob_backward_dims_and_refusals(e):
     refused(lambda: e.token_logprobs_backward(x, ids, row, None, row, bf16=True, into=zeros(e, 5, 100)))
 
 
+def test_widths_and_scales_beyond_the_kernels_are_refused(e):
+    c = Cache(e)
+    d = 65535
+    heads = 2**31 // d + 1                                                                  # columns behind 31 bits (of no rows)
+    wide = zeros(e, 0, (heads + 2) * d, BF16)
+    refused(lambda: e.rope_append_pages(PageShape(heads, 1, d, 1), (wide, (0, 0), (0, (heads + 2) * d)), None, None, zeros(e, 0, 1, I32), None,
+                                        c.table, zeros(e, 0, d, BF16), zeros(e, 0, d, BF16)))
+    q, p = zeros(e, 3, 128), zeros(e, 1, 3, I32)
+    c.attend(e, q=q, positions=p, scale=-1e20)
+    for scale in (1.1e20, -1.1e20, float("-inf")):
+        refused(lambda: c.attend(e, q=q, positions=p, scale=scale))
+    x, ids, row = zeros(e, 5, 100), zeros(e, 5, 1, I32), zeros(e, 5, 1)
+    for scale in (1e-20 * 1.01, 1e6):
+        e.token_logprobs(x, ids, scale)
+        e.token_logprobs_backward(x, ids, row, None, row, scale=scale)
+    refused(lambda: e.token_logprobs(x, ids, 1.1e6))
+    refused(lambda: e.token_logprobs_backward(x, ids, row, None, row, scale=1.1e6))
+
+
 def test_a_failed_launch_leaves_no_result(fake, e):
     c = Cache(e)
     x, q, p, ids, row = zeros(e, 3, 256, BF16), zeros(e, 3, 128), zeros(e, 1, 3, I32), zeros(e, 3, 1, I32), zeros(e, 3, 1)
