@@ -11,7 +11,7 @@ Tolerances, u = 2^-24, m the row's largest y = scale x:
 import numpy as np
 import pytest
 
-from metalium_rs_b200 import I32, SUM, COLS, TtError
+from metalium_rs_b200 import BF16, I32, SUM, COLS, TtError
 from oracle import oracle as orc
 
 pytestmark = pytest.mark.gpu
@@ -372,4 +372,37 @@ def test_results_into_buffers_and_replays(eng):
         assert all(np.array_equal(p, q) for p, q in zip(read(), want))
     eng.release_trace(trace)
     for i in into + [ix, ii, grad, one]:
+        eng.free(i)
+
+
+def test_offsets_behind_32_bits(fresh_eng):
+    eng = fresh_eng                                          # its memory goes back with it
+    # The last rows of logits of 2^32 elements and a few more, and their gradient.
+    rng = np.random.default_rng(18)
+    cols, tail = 50257, 5
+    rows = 2 ** 32 // cols + tail + 1
+    x = orc.to_bf16(logits(rng, tail, cols))
+    ids = np.full(rows, -1, np.int32)
+    ids[-tail:] = rng.integers(0, cols, tail)
+    whole = eng.zeros_dram((rows, cols), BF16)[0]
+    last = eng.slice_rows(whole, rows - tail, tail)[0]
+    eng.write_ptr(last, x.ctypes.data, x.size, 2)
+    eng.sync()
+    ii, one = up_i32(eng, ids, rows, 1), eng.upload(np.ones((rows, 1), np.float32), rows, 1)
+    got = eng.token_logprobs(whole, ii, 1.0, 3)
+    grad, _ = eng.token_logprobs_backward(whole, ii, got[2][0], got[1][0], one, one, bf16=True)
+    few, few_ids = eng.upload_bf16(x, tail, cols), up_i32(eng, ids[-tail:], tail, 1)
+    want = eng.token_logprobs(few, few_ids, 1.0, 3)
+    ends = eng.slice_rows(grad, rows - tail, tail)[0]
+    for (a, _), (b, _), width in zip(got, want, (1, 1, 1, 3, 3)):
+        a, b = eng.download_bits(a).reshape(rows, width), eng.download_bits(b).reshape(tail, width)
+        if a.dtype == np.uint32 and width == 3 and (b < cols).all():
+            assert np.array_equal(a[-tail:], b) and np.array_equal(a[0], [0, 1, 2])          # the columns
+        else:                                                                                 # summed in another order: few rows share blocks
+            assert np.all(np.abs(a[-tail:].view(np.float32) - b.view(np.float32)) <= 24 * (2 * 12 + 600) * U)   # twice, 1 + log 50257
+    ones = eng.upload(np.ones((tail, 1), np.float32), tail, 1)
+    lse, ent = (eng.slice_rows(got[i][0], rows - tail, tail)[0] for i in (2, 1))
+    few_grad, _ = eng.token_logprobs_backward(few, few_ids, lse, ent, ones, ones, bf16=True)
+    assert np.array_equal(eng.download_bf16(ends), eng.download_bf16(few_grad))
+    for i in [whole, last, ii, one, grad, few, few_ids, ends, ones, few_grad, lse, ent] + [i for i, _ in got + want]:
         eng.free(i)

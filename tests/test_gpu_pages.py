@@ -492,3 +492,51 @@ def test_append_and_attention_repeat_and_replay_bit_for_bit(eng):
     eng.release_trace(trace)
     for i in (it, ip, o) + state + second:
         eng.free(i)
+
+
+def test_offsets_behind_32_bits(fresh_eng):
+    eng = fresh_eng                                          # its memory goes back with it
+    # The last pages of pools of 2^32 elements and a few more: the bits of the same call on a small pool.
+    rng = np.random.default_rng(15)
+    shape, page, n, cols = PageShape(8, 8, 128, 64), 64, 3, 24 * 128
+    lengths, count = [100, 64, 3], 4
+    x = orc.to_bf16(rng.standard_normal((sum(lengths), cols)).astype(np.float32))
+    sequences = np.repeat(np.arange(n), lengths)
+    positions = np.concatenate([np.arange(m) for m in lengths])
+    small = np.array([[2, 0], [3, -1], [1, -1]], np.int32)
+    results = []
+    for pages in (count, 2 ** 32 // (page * 1024) + count):
+        table = np.where(small < 0, small, small + pages - count)
+        ik, iv = (eng.zeros_dram((pages * page, 1024), BF16)[0] for _ in range(2))
+        it, ip, js = up_i32(eng, table, *table.shape), up_i32(eng, positions, 1, len(x)), up_i32(eng, sequences, 1, len(x))
+        last = up_i32(eng, np.array(lengths) - 1, 1, n)
+        ix = eng.upload_bf16(x, *x.shape)
+        q, _ = eng.rope_append_pages(shape, (ix, (0, 0), x.shape), None, None, ip, js, it, ik, iv)
+        o, _ = eng.attention_pages(shape, (q, (0, 0), (n, 1024)), ik, iv, it, last, 0.09)
+        tail, _ = eng.slice_rows(ik, (pages - count) * page, count * page)
+        results.append((eng.download_bits(o), eng.download_bf16(tail)))
+        for i in (ik, iv, it, ip, js, last, ix, q, o, tail):
+            eng.free(i)
+    assert np.array_equal(results[0][0], results[1][0]) and np.array_equal(results[0][1], results[1][1])
+    assert np.abs(results[0][0].view(np.float32)).max() > 0.01
+
+
+def test_two_engines_at_once(eng, fresh_eng):
+    # Calls of two engines in turn, nothing waited for between them, are each engine's own.
+    rng = np.random.default_rng(16)
+    shape, lengths = PageShape(4, 2, 64, 16), [900, 33, 400]
+    table, pages = tables(rng, lengths, 16)
+    sides = []
+    for e in (eng, fresh_eng):
+        q, k, v = (rng.standard_normal((r, c)).astype(np.float32) for r, c in ((3, 256), (pages * 16, 128), (pages * 16, 128)))
+        ids = [e.upload(a, *a.shape) for a in (q, k, v)] + [up_i32(e, table, *table.shape), up_i32(e, np.array(lengths) - 1, 1, 3)]
+        alone, _ = e.attention_pages(shape, (ids[0], (0, 0), (3, 256)), *ids[1:], 0.125)
+        sides.append((e, ids, e.download_bits(alone), alone))
+    for _ in range(20):
+        outs = [e.attention_pages(shape, (ids[0], (0, 0), (3, 256)), *ids[1:], 0.125)[0] for e, ids, _, _ in sides]
+        for (e, _, want, _), o in zip(sides, outs):
+            assert np.array_equal(e.download_bits(o), want)
+            e.free(o)
+    for e, ids, _, alone in sides:
+        for i in ids + [alone]:
+            e.free(i)
