@@ -250,6 +250,7 @@ __global__ void __launch_bounds__(Form<KV, D>::THREADS, Form<KV, D>::BLOCKS) att
     // ---- the copies' side: the rows of the tile that is issued next
     Cursor ahead;
     seek(ahead, start);
+    Cursor here = ahead;                 // the run's other side: the tile that is summed next
     uint32_t to_issue = stop - start;
     int32_t row = -1;                    // lane % 16's pool row of the tile at `ahead`, -1: not attended
     const auto look_up = [&]() {
@@ -298,8 +299,6 @@ __global__ void __launch_bounds__(Form<KV, D>::THREADS, Form<KV, D>::BLOCKS) att
     for (int i = 0; i < a.stages; ++i) { issue_keys(); issue_values(); }
 
     // ---- the run's sequences, one after another
-    Cursor here;
-    seek(here, start);
     int stage = 0, piece = 0;
     for (uint32_t left = stop - start; left > 0; ++piece) {
       const uint32_t steps = left < here.tiles - here.tile ? left : here.tiles - here.tile;
