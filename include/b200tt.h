@@ -510,6 +510,15 @@ int32_t b200_token_logprobs_backward(b200_engine*, b200_buffer logits, b200_buff
                                      b200_buffer d_logprob, b200_buffer d_entropy, float scale, int32_t out_bf16,
                                      b200_buffer into, b200_buffer* out, uint64_t out_dims[2]);
 
+/* The four calls above with their arguments as 64-bit words, for bindings in which every argument of a foreign call has its cost
+ * (ctypes: 2.2 us for the append's fifteen, 1.0 for four and the packing).  `words` holds the arguments behind the engine
+ * in their order, each in a word of its own -- a shape as its address, a block as its five words, an integer
+ * zero-extended, a float's bits in the low half, the five ids of `into` one after another -- and behind them takes the
+ * results: `out` (1 or 5 words) and out_dims (2), written when the call succeeds.  n_words is the count of all of them: 19, 17,
+ * 16 and 12.  Another call or count is refused. */
+enum { B200_ROPE_APPEND_PAGES = 0, B200_ATTENTION_PAGES = 1, B200_TOKEN_LOGPROBS = 2, B200_TOKEN_LOGPROBS_BACKWARD = 3 };
+int32_t b200_serving_call(b200_engine*, int32_t call, uint64_t* words, uint64_t n_words);
+
 /* --- traces: server.rs:591 `begin_trace`, :595 `end_trace`, :650 `run_trace`, :660 `release_trace`.
  * Ops issued between begin and end are captured into a CUDA graph instead of running; a replay
  * runs them again on the same buffers.  Inputs are buffers made before the capture (refresh them

@@ -2,6 +2,7 @@
 // log probabilities of given tokens with their gradient.  Argument checks, results and launches only; the state is the
 // engine's (engine.h), the kernels are k_pages.cu's and k_logprob.cu's.
 #include <cmath>
+#include <cstring>
 
 #include "engine.h"
 #include "kernels.h"
@@ -15,12 +16,16 @@ typedef unsigned long long ull;
 // A buffer's memory, for the checks that a result written over a caller's buffer shares none of it.
 struct Span { const char* at; uint64_t bytes; };
 Span span_of(const Buf* b) { return Span{(const char*)b->ptr, b->rows * b->cols * elem_bytes(b->elem)}; }
+struct Spans {
+  Span list[12];                         // a call has at most ten operands
+  size_t n = 0;
+  void push_back(const Span& s) { list[n++] = s; }
+};
 bool meet(const Span& a, const Span& b) { return a.bytes && b.bytes && a.at < b.at + b.bytes && b.at < a.at + a.bytes; }
 
 // Where a result goes: `into`, checked, or a new buffer.  `made` says whether it is to be dropped when the call fails.
 struct Result { void* ptr = nullptr; b200_buffer id = 0; bool made = false; };
-int result_of(b200_engine* e, b200_buffer into, uint64_t rows, uint64_t cols, int elem, const std::vector<Span>& inputs, const char* what,
-              Result* r) {
+int result_of(b200_engine* e, b200_buffer into, uint64_t rows, uint64_t cols, int elem, const Spans& inputs, const char* what, Result* r) {
   Buf* b = nullptr;
   if (!into) {
     int st = e->new_buffer(rows, cols, elem, &r->id, &b);
@@ -35,8 +40,8 @@ int result_of(b200_engine* e, b200_buffer into, uint64_t rows, uint64_t cols, in
     return e->fail(B200_UNSUPPORTED, "%s: the result is [%llu, %llu] of element %d, `into` is [%llu, %llu] of %d", what, (ull)rows, (ull)cols,
                    elem, (ull)b->rows, (ull)b->cols, b->elem);
   if (reinterpret_cast<uintptr_t>(b->ptr) & 15) return e->fail(B200_UNSUPPORTED, "%s: `into` does not start at a 16-byte address", what);
-  for (const Span& s : inputs)
-    if (meet(s, span_of(b))) return e->fail(B200_UNSUPPORTED, "%s: `into` shares memory with another buffer of the call", what);
+  for (size_t i = 0; i < inputs.n; ++i)
+    if (meet(inputs.list[i], span_of(b))) return e->fail(B200_UNSUPPORTED, "%s: `into` shares memory with another buffer of the call", what);
   r->ptr = b->ptr;
   r->id = into;
   return B200_OK;
@@ -66,7 +71,7 @@ int int_list(b200_engine* e, b200_buffer id, uint64_t n, Buf** b, const char* na
 
 // The cache both calls read: shape, pages, table.
 int page_view(b200_engine* e, const b200_page_shape* shape, b200_buffer key_pages, b200_buffer value_pages, b200_buffer page_table,
-              PageView* v, std::vector<Span>* spans, const char* what) {
+              PageView* v, Spans* spans, const char* what) {
   Buf *K = nullptr, *V = nullptr, *T = nullptr;
   int st = e->need(key_pages, &K, what);
   if (!st) st = e->need(value_pages, &V, what);
@@ -129,7 +134,7 @@ int32_t b200_rope_append_pages(b200_engine* e, const b200_page_shape* shape, con
   const char* what = "rope_append_pages";
   cudaSetDevice(e->device);
   AppendArgs g;
-  std::vector<Span> spans;
+  Spans spans;
   Buf *X = nullptr, *P = nullptr, *S = nullptr, *C = nullptr, *N = nullptr;
   int st = page_view(e, shape, key_pages, value_pages, page_table, &g.cache, &spans, what);
   if (!st) st = float_block(e, qkv, &g.qkv, &X, what);
@@ -159,8 +164,8 @@ int32_t b200_rope_append_pages(b200_engine* e, const b200_page_shape* shape, con
   spans.push_back(span_of(X)); spans.push_back(span_of(P));
   if (S) spans.push_back(span_of(S));
   // the pages are written while the other operands are read
-  for (size_t i = 2; i < spans.size(); ++i)
-    if (meet(spans[0], spans[i]) || meet(spans[1], spans[i])) return e->fail(B200_UNSUPPORTED, "%s: the pages share memory with another operand", what);
+  for (size_t i = 2; i < spans.n; ++i)
+    if (meet(spans.list[0], spans.list[i]) || meet(spans.list[1], spans.list[i])) return e->fail(B200_UNSUPPORTED, "%s: the pages share memory with another operand", what);
   const uint64_t cols = ((uint64_t)shape->heads + (keys_out ? shape->kv_heads : 0)) * d;
   Result r;
   st = result_of(e, into, n, cols, out_bf16 ? B200_BF16 : B200_F32, spans, what, &r);
@@ -180,7 +185,7 @@ int32_t b200_attention_pages(b200_engine* e, const b200_page_shape* shape, const
   const char* what = "attention_pages";
   cudaSetDevice(e->device);
   AttnPagesArgs g;
-  std::vector<Span> spans;
+  Spans spans;
   Buf *Q = nullptr, *P = nullptr;
   int st = page_view(e, shape, key_pages, value_pages, page_table, &g.cache, &spans, what);
   if (!st) st = float_block(e, q, &g.q, &Q, what);
@@ -227,7 +232,8 @@ int32_t b200_token_logprobs(b200_engine* e, b200_buffer logits, b200_buffer ids,
   LogprobArgs g;
   g.logits = X->ptr; g.bf16 = X->elem == B200_BF16; g.rows = rows; g.cols = cols;
   g.ids = (const int32_t*)I->ptr; g.scale = scale; g.top = top; g.err = e->d_err;
-  std::vector<Span> spans = {span_of(X), span_of(I)};
+  Spans spans;
+  spans.push_back(span_of(X)); spans.push_back(span_of(I));
   Result r[5];
   const int parts = top ? 5 : 3;
   for (int i = 0; i < parts; ++i) {
@@ -260,7 +266,8 @@ int32_t b200_token_logprobs_backward(b200_engine* e, b200_buffer logits, b200_bu
   if (!st && d_entropy) st = row_values(e, entropy, rows, &H, "entropy", what);
   if (st) return st;
   if (!good_scale(scale)) return e->fail(B200_UNSUPPORTED, "%s: the scale %g is not within 1e-20 .. 1e6", what, scale);
-  std::vector<Span> spans = {span_of(X), span_of(I), span_of(L), span_of(G)};
+  Spans spans;
+  for (const Buf* b : {X, I, L, G}) spans.push_back(span_of(b));
   if (GH) { spans.push_back(span_of(GH)); spans.push_back(span_of(H)); }
   Result r;
   st = result_of(e, into, rows, cols, out_bf16 ? B200_BF16 : B200_F32, spans, what, &r);
@@ -275,6 +282,33 @@ int32_t b200_token_logprobs_backward(b200_engine* e, b200_buffer logits, b200_bu
   *out = r.id;
   set_dims(out_dims, rows, cols);
   return B200_OK;
+}
+
+int32_t b200_serving_call(b200_engine* e, int32_t call, uint64_t* w, uint64_t n_words) {
+  const uint64_t counts[4] = {19, 17, 16, 12};
+  if (call < 0 || call > 3 || n_words != counts[call])
+    return e->fail(B200_UNSUPPORTED, "serving_call: call %d of %llu words", call, (ull)n_words);
+  const auto f32_of = [](uint64_t word) {
+    const uint32_t bits = (uint32_t)word;
+    float f;
+    memcpy(&f, &bits, 4);
+    return f;
+  };
+  const b200_page_shape* shape = reinterpret_cast<const b200_page_shape*>(w[0]);
+  const b200_block_arg block = {w[1], {w[2], w[3]}, {w[4], w[5]}};
+  switch (call) {
+    case B200_ROPE_APPEND_PAGES:
+      return b200_rope_append_pages(e, shape, &block, w[6], w[7], w[8], w[9], w[10], w[11], w[12], (int32_t)w[13], (int32_t)w[14], w[15],
+                                    (b200_buffer*)&w[16], &w[17]);
+    case B200_ATTENTION_PAGES:
+      return b200_attention_pages(e, shape, &block, w[6], w[7], w[8], w[9], (uint32_t)w[10], f32_of(w[11]), (int32_t)w[12], w[13],
+                                  (b200_buffer*)&w[14], &w[15]);
+    case B200_TOKEN_LOGPROBS:
+      return b200_token_logprobs(e, w[0], w[1], f32_of(w[2]), (uint32_t)w[3], (const b200_buffer*)&w[4], (b200_buffer*)&w[9], &w[14]);
+    default:
+      return b200_token_logprobs_backward(e, w[0], w[1], w[2], w[3], w[4], w[5], f32_of(w[6]), (int32_t)w[7], w[8], (b200_buffer*)&w[9],
+                                          &w[10]);
+  }
 }
 
 }  // extern "C"

@@ -120,14 +120,6 @@ def _prepare(_lib: C.CDLL) -> C.CDLL:
         _lib.b200_traffic_get.restype = None
         _lib.b200_last_oom.restype = None
         _lib.b200_release_trace.restype = None
-        # A step's calls: with their argument types declared they take plain numbers, at a third of the cost of wrapping each
-        u64, i32, u32, f32, p = C.c_uint64, C.c_int32, C.c_uint32, C.c_float, C.c_void_p
-        for name, types in (("b200_rope_append_pages", [p, p, p] + [u64] * 7 + [i32, i32, u64, p, p]),
-                            ("b200_attention_pages", [p, p, p] + [u64] * 4 + [u32, f32, i32, u64, p, p]),
-                            ("b200_token_logprobs", [p, u64, u64, f32, u32, p, p, p]),
-                            ("b200_token_logprobs_backward", [p] + [u64] * 6 + [f32, i32, u64, p, p])):
-            if hasattr(_lib, name):
-                getattr(_lib, name).argtypes = types
     return _lib
 
 
@@ -153,14 +145,16 @@ def _block(b) -> "BlockArg":
     return BlockArg(bid, (C.c_uint64 * 2)(*at), (C.c_uint64 * 2)(*dims))
 
 
-_BLOCK = struct.Struct("=5Q")
+# A generation step's calls go as words (`b200_serving_call`): in one piece they cost half of what ctypes takes for each argument.
+_WORDS = (struct.Struct("=19Q"), struct.Struct("=11QfI5Q"), struct.Struct("=2QfI13Q"), struct.Struct("=6QfI5Q"))
+_COUNTS = tuple(C.c_uint64(w.size // 8) for w in _WORDS)
+_RESULT, _RESULTS = struct.Struct("=3Q"), struct.Struct("=6Q")
 
 
-def _block_ptr(b):
-    """A block for a step's call: the bytes of a `BlockArg`, without making one."""
+def _block_words(b):
     if isinstance(b, BlockArg):
-        return C.byref(b)
-    return _BLOCK.pack(b[0], *b[1], *b[2])
+        return b.id, b.at[0], b.at[1], b.dims[0], b.dims[1]
+    return b[0], *b[1], *b[2]
 
 
 Out = Tuple[int, Tuple[int, int]]
@@ -184,6 +178,8 @@ class CudaEngine:
             raise TtError(st, buf.value.decode())
         self.device = device
         self.profiling = False
+        self._words = C.create_string_buffer(8 * 19)         # one driving thread an engine: one call at a time
+        self._words_at = C.c_void_p(C.addressof(self._words))
 
     # -- plumbing ------------------------------------------------------------
     def close(self):
@@ -214,6 +210,11 @@ class CudaEngine:
         dims = (C.c_uint64 * 2)()
         self._check(fn(self._e, *args, C.byref(out), dims))
         return out.value, (dims[0], dims[1])
+
+    def _serving_call(self, call: int, at: int) -> Out:
+        self._check(self._lib.b200_serving_call(self._e, call, self._words_at, _COUNTS[call]))
+        out, rows, cols = _RESULT.unpack_from(self._words, at)
+        return out, (rows, cols)
 
     # -- capabilities (server.rs:53,75,240) --------------------------------------
     def supports_dram(self) -> bool:
@@ -728,8 +729,9 @@ class CudaEngine:
         """RoPE on a projection's query and key heads and the cache write as one pass (`b200_rope_append_pages`): qkv is a
         block [n, (heads + 2 kv_heads) head_dim]; row i is the token at positions[i] of sequence sequences[i] (None: of
         sequence i), -1 a padding row.  Returns the rotated query heads, with `keys` the rotated key heads behind them."""
-        return self._call(self._lib.b200_rope_append_pages, C.byref(shape), _block_ptr(qkv), cos or 0, sin or 0, positions, sequences or 0,
-                          page_table, key_pages, value_pages, 1 if keys else 0, 1 if bf16 else 0, into)
+        _WORDS[0].pack_into(self._words, 0, C.addressof(shape), *_block_words(qkv), cos or 0, sin or 0, positions, sequences or 0, page_table,
+                            key_pages, value_pages, 1 if keys else 0, 1 if bf16 else 0, into, 0, 0, 0)
+        return self._serving_call(0, 128)
 
     def attention_pages(self, shape: "PageShape", q, key_pages: int, value_pages: int, page_table: int, positions: int, scale: float,
                         window: int = 0, bf16: bool = False, into: int = 0) -> Out:
@@ -738,24 +740,30 @@ class CudaEngine:
         keeps the last `window` positions.  Returns [n, heads head_dim]."""
         if not 0 <= window < 2**32:
             raise ValueError("a window is 0 (every position) or a count of positions")
-        return self._call(self._lib.b200_attention_pages, C.byref(shape), _block_ptr(q), key_pages, value_pages, page_table, positions,
-                          window, scale, 1 if bf16 else 0, into)
+        _WORDS[1].pack_into(self._words, 0, C.addressof(shape), *_block_words(q), key_pages, value_pages, page_table, positions, window,
+                            scale, 0, 1 if bf16 else 0, into, 0, 0, 0)
+        return self._serving_call(1, 112)
 
     def token_logprobs(self, logits: int, ids: int, scale: float = 1.0, top: int = 0, into: Optional[Sequence[int]] = None):
         """(logprob, entropy, lse) [rows, 1] of the given tokens under softmax(scale * logits), and with `top` > 0 the
         (columns, log probabilities) [rows, top] of the largest logits (`b200_token_logprobs`): three or five (id, dims)."""
         if not 0 <= top < 2**32:
             raise ValueError("the alternatives are a count")
-        out, dims = (C.c_uint64 * 5)(), (C.c_uint64 * 2)()
-        self._check(self._lib.b200_token_logprobs(self._e, logits, ids, scale, top, (C.c_uint64 * 5)(*into) if into is not None else None, out, dims))
-        rows = dims[0]
-        return [(out[i], (rows, 1 if i < 3 else top)) for i in range(5 if top else 3)]
+        if into is None:
+            into = ()
+        elif len(into) > 5:
+            raise ValueError("five results at most")
+        _WORDS[2].pack_into(self._words, 0, logits, ids, scale, 0, top, *into, *(0,) * (12 - len(into)))
+        self._check(self._lib.b200_serving_call(self._e, 2, self._words_at, _COUNTS[2]))
+        a, b, c, d, e, rows = _RESULTS.unpack_from(self._words, 72)
+        one = (rows, 1)
+        return [(a, one), (b, one), (c, one), (d, (rows, top)), (e, (rows, top))] if top else [(a, one), (b, one), (c, one)]
 
     def token_logprobs_backward(self, logits: int, ids: int, lse: int, entropy: Optional[int], d_logprob: int, d_entropy: Optional[int] = None,
                                 scale: float = 1.0, bf16: bool = False, into: int = 0) -> Out:
         """The gradient of `token_logprobs`' log probabilities (and, with d_entropy, entropies) with respect to the logits."""
-        return self._call(self._lib.b200_token_logprobs_backward, logits, ids, lse, entropy or 0, d_logprob, d_entropy or 0, scale,
-                          1 if bf16 else 0, into)
+        _WORDS[3].pack_into(self._words, 0, logits, ids, lse, entropy or 0, d_logprob, d_entropy or 0, scale, 0, 1 if bf16 else 0, into, 0, 0, 0)
+        return self._serving_call(3, 72)
 
     def set_matmul_sm_limit(self, sms: int):
         """Tensor-core products use at most `sms` SMs (0 = all): room for a collective beside them."""

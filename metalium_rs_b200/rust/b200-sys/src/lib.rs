@@ -108,6 +108,7 @@ extern "C" {
     pub fn b200_attention_pages(a0: *mut b200_engine, shape: *const b200_page_shape, q: *const b200_block_arg, key_pages: u64, value_pages: u64, page_table: u64, positions: u64, window: u32, scale: f32, out_bf16: i32, into: u64, out: *mut u64, out_dims: *mut u64) -> i32;
     pub fn b200_token_logprobs(a0: *mut b200_engine, logits: u64, ids: u64, scale: f32, top: u32, into: *const u64, out: *mut u64, out_dims: *mut u64) -> i32;
     pub fn b200_token_logprobs_backward(a0: *mut b200_engine, logits: u64, ids: u64, lse: u64, entropy: u64, d_logprob: u64, d_entropy: u64, scale: f32, out_bf16: i32, into: u64, out: *mut u64, out_dims: *mut u64) -> i32;
+    pub fn b200_serving_call(a0: *mut b200_engine, call: i32, words: *mut u64, n_words: u64) -> i32;
     pub fn b200_begin_trace(a0: *mut b200_engine) -> i32;
     pub fn b200_end_trace(a0: *mut b200_engine, trace: *mut u64) -> i32;
     pub fn b200_run_trace(a0: *mut b200_engine, trace: u64) -> i32;

@@ -257,3 +257,34 @@ def test_the_calls_are_captured_into_a_trace(e):
     assert len(e.trace_ops(t)) == 3
     e.run_trace(t)
     e.release_trace(t)
+
+
+def test_calls_as_words(fake, e):
+    """Every call as words is the call with its arguments: results, dims and refusals; other words are refused."""
+    w, u64 = (C.c_uint64 * 19)(), C.c_uint64
+    send = lambda call, n, *words: fake.b200_serving_call(e._e, C.c_int32(call), w, u64(n)) if not w.__setitem__(slice(0, len(words)), words) else None  # noqa: E731
+    for call, n in ((-1, 19), (4, 12), (0, 18), (1, 19), (2, 17), (3, 11)):
+        assert send(call, n) == 2
+    c = Cache(e)
+    x, p, q = zeros(e, 3, 256, BF16), zeros(e, 1, 3, I32), zeros(e, 3, 128)
+    at = C.addressof(c.shape)
+    assert send(0, 19, at, x, 0, 0, 3, 256, c.cos, c.sin, p, 0, c.table, c.keys, c.values, 1, 1, 0, 0, 0, 0) == 0
+    assert (w[17], w[18]) == (3, 192) and e.dims_of(w[16]) == ((3, 192), BF16)
+    half = int(np.float32(0.5).view(np.uint32))
+    assert send(1, 17, at, q, 0, 0, 3, 128, c.keys, c.values, c.table, p, 7, half, 0, q, 0, 0, 0) == 2   # into one of the operands
+    out = zeros(e, 3, 128)
+    assert send(1, 17, at, q, 0, 0, 3, 128, c.keys, c.values, c.table, p, 7, half, 0, out, 0, 0, 0) == 0
+    assert (w[14], w[15], w[16]) == (out, 3, 128)
+    logits, ids, row = zeros(e, 5, 100), zeros(e, 5, 1, I32), zeros(e, 5, 1)
+    assert send(2, 16, logits, ids, half, 4, 0, 0, row, 0, 0) == 0
+    assert w[11] == row and [e.dims_of(w[i])[0] for i in (9, 10, 12, 13)] == [(5, 1), (5, 1), (5, 4), (5, 4)] and (w[14], w[15]) == (5, 1)
+    assert send(2, 16, logits, ids, half, 4, 31337, 0, 0, 0, 0) == 5
+    assert send(3, 12, logits, ids, row, row, row, row, half, 1, 0) == 0
+    assert e.dims_of(w[9]) == ((5, 100), BF16) and (w[10], w[11]) == (5, 100)
+    got = e.token_logprobs(logits, ids, top=3, into=[row])                                  # the others are new
+    assert got[0][0] == row and len(got) == 5
+    with pytest.raises(ValueError):
+        e.token_logprobs(logits, ids, into=[0] * 6)
+    from metalium_rs_b200.engine import BlockArg
+    block = BlockArg(q, (u64 * 2)(0, 0), (u64 * 2)(3, 128))
+    assert e.attention_pages(c.shape, block, c.keys, c.values, c.table, p, 0.5)[1] == (3, 128)
