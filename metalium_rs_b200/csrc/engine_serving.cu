@@ -206,10 +206,11 @@ int32_t b200_attention_pages(b200_engine* e, const b200_page_shape* shape, const
   int launches = 0;
   void* scratch = nullptr;
   uint64_t got = 0;
-  st = n ? e->alloc(attention_pages_scratch_bytes(g), &scratch, &got) : B200_OK;
+  const size_t bytes = n ? attention_pages_scratch_bytes(g) : 0;
+  st = bytes ? e->alloc(bytes, &scratch, &got) : B200_OK;
   if (st) { undo(e, r); return st; }
   const cudaError_t ce = launch_attention_pages(g, scratch, &launches, e->stream);
-  if (n) e->release(scratch, got);
+  if (bytes) e->release(scratch, got);
   st = e->launched(ce, what, launches);
   if (st) { undo(e, r); return st; }
   *out = r.id;

@@ -8,7 +8,9 @@
 // row's heads are read together (a row is one piece of memory).  A run may end inside a sequence and the next one goes on
 // there: a warp writes the results of sequences that lie in its run whole, and (maximum, sum, rows) of the at most two that do
 // not, which a second kernel joins.  The lengths are on the device, so the list is made there, from a prefix sum.  After that
-// sum no warp waits for another.
+// sum no warp waits for another.  Where the table leaves room for short sequences only, there is neither list nor second
+// kernel: a block, or a cluster of up to eight, has a (sequence, head) to itself, its warps equal shares of the tiles, and
+// joins them from shared memory (`cut_of` says when).
 //
 // A warp's pipeline: it copies its 16 keys and 16 values of a tile to its own shared memory by 16-byte asynchronous copies, as
 // many tiles ahead as it has room for (the place of a tile's keys is filled again as soon as its scores are taken, that of its
@@ -58,6 +60,7 @@ struct Form {
 constexpr uint32_t MAX_SEQUENCES = 512;  // a launch's; its prefix sums lie in shared memory
 constexpr int MAX_STAGES = 4;
 constexpr int HEADS = 8;                 // query heads a warp
+constexpr int CLUSTER = 8;               // blocks that share a (sequence, job), at most
 
 struct AttnPlan {
   AttnPagesArgs g;
@@ -67,6 +70,7 @@ struct AttnPlan {
   uint32_t jobs;                         // kv_heads * row_tiles
   uint32_t runs, slot;                   // runs the tiles are cut into; floats of a piece
   int stages;
+  int together;                          // the warps of a cluster of so many blocks share one (sequence, job) and join it themselves; 0: runs
   float scale_log2;
   float* part;                           // [runs][jobs][2] pieces: [rows][D], then (maximum, sum) a row in four floats
   uint32_t* prefix;                      // [n + 1], for the join
@@ -188,7 +192,7 @@ __global__ void __launch_bounds__(Form<KV, D>::THREADS, Form<KV, D>::BLOCKS) att
   unsigned char* stages = smem + F::prefix_bytes(n) + warp * a.stages * F::STAGE;
 
   // ---- the tile list: a prefix sum over the sequences; rows of sequences without positions are zero
-  {
+  if (!a.together) {
     const uint32_t each = (n + F::THREADS - 1) / F::THREADS, first = tid * each;
     uint32_t sum = 0;
     for (uint32_t s = first; s < first + each && s < n; ++s) {
@@ -211,13 +215,14 @@ __global__ void __launch_bounds__(Form<KV, D>::THREADS, Form<KV, D>::BLOCKS) att
     if (tid == F::THREADS - 1) prefix[n] = before + sum;
     __syncthreads();
   }
-  const uint32_t total = prefix[n];
-  if (blockIdx.x == 0)
-    for (uint32_t s = tid; s <= n; s += F::THREADS) a.prefix[s] = prefix[s];
-  const uint32_t out_cols = cache.heads * D;
-  for (uint32_t s = blockIdx.x; s < n; s += gridDim.x)
-    if (prefix[s] == prefix[s + 1])
-      for (uint32_t j = tid; j < out_cols; j += F::THREADS) store_float(g.out, (uint64_t)s * out_cols + j, g.out_bf16, 0.f);
+  const uint32_t total = a.together ? 0 : prefix[n], out_cols = cache.heads * D;
+  if (!a.together) {
+    if (blockIdx.x == 0)
+      for (uint32_t s = tid; s <= n; s += F::THREADS) a.prefix[s] = prefix[s];
+    for (uint32_t s = blockIdx.x; s < n; s += gridDim.x)
+      if (prefix[s] == prefix[s + 1])
+        for (uint32_t j = tid; j < out_cols; j += F::THREADS) store_float(g.out, (uint64_t)s * out_cols + j, g.out_bf16, 0.f);
+  }
 
   const auto enter = [&](Cursor& c) {    // the bounds of sequence c.s
     uint32_t count;
@@ -239,19 +244,32 @@ __global__ void __launch_bounds__(Form<KV, D>::THREADS, Form<KV, D>::BLOCKS) att
   const uint32_t ld = cache.kv_heads * D * (uint32_t)sizeof(KV);              // bytes of a pool row
   const uint32_t to = (uint32_t)__cvta_generic_to_shared(stages) + (lane % F::LANES) * 16;
 
-  const uint32_t tasks = a.runs * a.jobs;
+  uint32_t rank = 0;                     // this block's in its cluster
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+  const uint32_t tasks = a.together ? gridDim.x * F::WARPS : a.runs * a.jobs;
   for (uint32_t task = blockIdx.x * F::WARPS + warp; task < tasks; task += gridDim.x * F::WARPS) {   // the same for a warp's lanes
-    const uint32_t run = task / a.jobs, job = task % a.jobs;
-    const uint32_t start = run_start(total, run, a.runs), stop = run_start(total, run + 1, a.runs);
-    if (start >= stop) continue;
+    uint32_t job, count;                 // its tiles: `count` of them from `ahead`
+    Cursor ahead;
+    if (a.together) {                    // a share of one sequence's
+      job = blockIdx.x / a.together % a.jobs;
+      ahead.s = blockIdx.x / a.together / a.jobs;
+      enter(ahead);
+      const uint32_t warps = a.together * F::WARPS, share = (ahead.tiles + warps - 1) / warps;
+      ahead.tile = (rank * F::WARPS + warp) * share;
+      count = ahead.tile < ahead.tiles ? min(share, ahead.tiles - ahead.tile) : 0;
+    } else {
+      const uint32_t run = task / a.jobs, start = run_start(total, run, a.runs), stop = run_start(total, run + 1, a.runs);
+      if (start >= stop) continue;
+      job = task % a.jobs;
+      count = stop - start;
+      seek(ahead, start);
+    }
     const uint32_t kvh = job / a.row_tiles, r0 = job % a.row_tiles * HEADS;
     const uint32_t rows = a.group - r0 < HEADS ? a.group - r0 : HEADS, head0 = kvh * a.group + r0;
 
     // ---- the copies' side: the rows of the tile that is issued next
-    Cursor ahead;
-    seek(ahead, start);
     Cursor here = ahead;                 // the run's other side: the tile that is summed next
-    uint32_t to_issue = stop - start;
+    uint32_t to_issue = count;
     int32_t row = -1;                    // lane % 16's pool row of the tile at `ahead`, -1: not attended
     const auto look_up = [&]() {
       row = -1;
@@ -289,8 +307,8 @@ __global__ void __launch_bounds__(Form<KV, D>::THREADS, Form<KV, D>::BLOCKS) att
     const auto issue_values = [&]() {
       if (to_issue) {
         copy(to + issue_stage * F::STAGE + 16 * F::K_PITCH, value_at, F::V_PITCH);
+        if (++ahead.tile == ahead.tiles && to_issue > 1) next_sequence(ahead);
         --to_issue;
-        if (++ahead.tile == ahead.tiles) next_sequence(ahead);
         look_up();
       }
       cp_async_commit();
@@ -300,7 +318,7 @@ __global__ void __launch_bounds__(Form<KV, D>::THREADS, Form<KV, D>::BLOCKS) att
 
     // ---- the run's sequences, one after another
     int stage = 0, piece = 0;
-    for (uint32_t left = stop - start; left > 0; ++piece) {
+    for (uint32_t left = count; left > 0; ++piece) {
       const uint32_t steps = left < here.tiles - here.tile ? left : here.tiles - here.tile;
       const bool whole = here.tile == 0 && steps == here.tiles;
 
@@ -512,7 +530,7 @@ __global__ void __launch_bounds__(Form<KV, D>::THREADS, Form<KV, D>::BLOCKS) att
       l += __shfl_xor_sync(0xffffffffu, l, 1);
       l += __shfl_xor_sync(0xffffffffu, l, 2);
       if (gr < (int)rows) {
-        if (whole) {
+        if (whole && !a.together) {
           const float den = l < FLT_MIN ? FLT_MIN : l;
           const uint64_t at = (uint64_t)here.s * out_cols + (uint64_t)(head0 + gr) * D + 2 * t4;
 #pragma unroll
@@ -526,7 +544,8 @@ __global__ void __launch_bounds__(Form<KV, D>::THREADS, Form<KV, D>::BLOCKS) att
             else *reinterpret_cast<float2*>(reinterpret_cast<float*>(g.out) + at + j * 8) = make_float2(u, v);
           }
         } else {
-          float* part = a.part + ((uint64_t)task * 2 + (piece ? 1 : 0)) * a.slot;
+          // (a warp's own tiles are behind it: their room takes its part where the block joins them)
+          float* part = a.together ? reinterpret_cast<float*>(stages) : a.part + ((uint64_t)task * 2 + (piece ? 1 : 0)) * a.slot;
 #pragma unroll
           for (int j = 0; j < D / 8; ++j) {
             float u = o[j][0], v = o[j][1];
@@ -538,10 +557,65 @@ __global__ void __launch_bounds__(Form<KV, D>::THREADS, Form<KV, D>::BLOCKS) att
       }
       left -= steps;
       here.tile += steps;
-      if (here.tile == here.tiles) next_sequence(here);
+      if (here.tile == here.tiles && left > 0) next_sequence(here);
     }
     cp_async_wait(0);
     __syncwarp();
+    if (a.together) {                    // once a block: its warps' parts, then its cluster's, each in their order
+      __syncthreads();
+      const uint32_t warps = a.together * F::WARPS, share = (here.tiles + warps - 1) / warps, all = share ? (here.tiles + share - 1) / share : 0;
+      const uint32_t held = all > rank * F::WARPS ? min(all - rank * F::WARPS, (uint32_t)F::WARPS) : 0;   // of `all` warps with tiles, this block's
+      const uint32_t ml = a.slot / (D + 4) * D;
+      const uint64_t at = (uint64_t)here.s * out_cols + (uint64_t)head0 * D;
+      unsigned char* parts = smem + F::prefix_bytes(n);
+      float* mine = reinterpret_cast<float*>(parts + F::STAGE);       // behind the first warp's part
+      for (uint32_t j = tid; j < rows * D; j += F::THREADS) {
+        const uint32_t r = j / D;
+        float top = -FLT_MAX, v = 0.f, den = 0.f;
+        for (uint32_t w = 0; w < held; ++w) top = fmaxf(top, reinterpret_cast<const float*>(parts + w * a.stages * F::STAGE)[ml + r * 4]);
+        for (uint32_t w = 0; w < held; ++w) {
+          const float* p = reinterpret_cast<const float*>(parts + w * a.stages * F::STAGE);
+          const float f = exp2_fast(p[ml + r * 4] - top);
+          den = fmaf(p[ml + r * 4 + 1], f, den);
+          v = fmaf(p[j], f, v);
+        }
+        if (a.together == 1) store_float(g.out, at + j, g.out_bf16, v / (den < FLT_MIN ? FLT_MIN : den));
+        else {
+          mine[j] = v;
+          if (j % D == 0) { mine[ml + r * 4] = top; mine[ml + r * 4 + 1] = den; }
+        }
+      }
+      if (a.together > 1) {
+        asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+        const uint32_t own = (uint32_t)__cvta_generic_to_shared(mine), blocks = (all + F::WARPS - 1) / F::WARPS;
+        const auto theirs = [&](uint32_t block, uint32_t i) {
+          uint32_t at_block;
+          float x;
+          asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at_block) : "r"(own + i * 4), "r"(block));
+          asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(at_block) : "memory");
+          return x;
+        };
+        for (uint32_t j = rank * F::THREADS + tid; j < rows * D; j += a.together * F::THREADS) {
+          const uint32_t r = j / D;
+          float tops[CLUSTER], dens[CLUSTER], values[CLUSTER], top = -FLT_MAX, v = 0.f, den = 0.f;
+#pragma unroll
+          for (uint32_t i = 0; i < CLUSTER; ++i) {
+            tops[i] = -FLT_MAX; dens[i] = values[i] = 0.f;
+            if (i < blocks) { tops[i] = theirs(i, ml + r * 4); dens[i] = theirs(i, ml + r * 4 + 1); values[i] = theirs(i, j); }
+          }
+#pragma unroll
+          for (uint32_t i = 0; i < CLUSTER; ++i) top = fmaxf(top, tops[i]);
+#pragma unroll
+          for (uint32_t i = 0; i < CLUSTER; ++i) {
+            const float f = exp2_fast(tops[i] - top);
+            den = fmaf(dens[i], f, den);
+            v = fmaf(values[i], f, v);
+          }
+          store_float(g.out, at + j, g.out_bf16, v / (den < FLT_MIN ? FLT_MIN : den));
+        }
+        asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");   // no block leaves while it is read
+      }
+    }
   }
 }
 
@@ -632,8 +706,8 @@ int sm_count() {
 }
 
 // How a launch of `n` sequences is cut, from the shapes alone.
-struct Cut { uint64_t n; uint32_t group, row_tiles, jobs, runs, slot, workers; uint64_t tiles; };
-Cut cut_of(const AttnPagesArgs& g, uint64_t left, int dim, int workers) {
+struct Cut { uint64_t n; uint32_t group, row_tiles, jobs, runs, slot, workers; uint64_t tiles; int together; };
+Cut cut_of(const AttnPagesArgs& g, uint64_t left, int dim, int workers, int warps) {
   Cut c;
   c.group = g.cache.heads / g.cache.kv_heads;
   c.row_tiles = (c.group + HEADS - 1) / HEADS;
@@ -645,6 +719,18 @@ Cut cut_of(const AttnPagesArgs& g, uint64_t left, int dim, int workers) {
   c.tiles = (positions + 15) / 16;                           // a sequence's, at most (below 2^28)
   c.n = left < MAX_SEQUENCES ? left : MAX_SEQUENCES;
   if (c.tiles && c.n > 0xffffffffull / c.tiles) c.n = 0xffffffffull / c.tiles;
+  // Together: the second launch, the list and the sums before it cost 3 to 6 us, an unequal share of the work costs its length.
+  // So where a (sequence, job) can have blocks of its own, as many as leave each warp two tiles if there is room for them
+  // (7/8 of it: clusters do not fill every SM), and then no warp has more than so many tiles: half an F32 cache's, whose tile
+  // takes longer, and half where the blocks leave a quarter of the GPU free, which runs would use.  us by runs / together, 32
+  // heads of 128 over 8: one sequence of 100 10.4 / 8.6, of 2,000 13.7 / 12.6, of 4,000 15.9 / 16.8; 8 of 5 to 600 13.9 / 12.5, to
+  // 4,000 27.8 / 27.8; 37 to 600 25.0 / 20.2, to 2,000 46.2 / 43.2, to 4,000 71.9 / 75.6; F32, 8 heads of 96, 8 to 1,000 15.9 / 14.0,
+  // to 4,000 31.0 / 36.7.
+  const uint64_t teams = c.n * c.jobs, resident = (uint64_t)workers / warps;
+  c.together = teams <= resident;
+  while (c.together && c.together < CLUSTER && teams * c.together * 2 <= resident * 7 / 8 && c.tiles > 2ull * c.together * warps) c.together *= 2;
+  const uint64_t most = (g.cache.bf16 ? 8 : 4) * (teams * c.together * 4 >= resident * 3 ? 2 : 1);
+  if (c.tiles > most * c.together * warps) c.together = 0;
   // Runs: as many as give every warp one (run, head).  With so many heads that a warp more or less in that division weighs,
   // the count whose last round of warps is fullest (8 sequences to 1,000, 600 heads of 64: 183 us, by one run a head 198).
   uint32_t runs = c.jobs < c.workers ? c.workers / c.jobs : 1;
@@ -671,7 +757,8 @@ cudaError_t attention_form(const AttnPagesArgs& g, void* scratch, int* launches,
   cudaError_t e = ensure_dynamic_smem((const void*)attention_pages_kernel<KV, D, QP, EXACT>, limit);
   if (e != cudaSuccess) return e;
   for (uint64_t at = 0; at < g.n;) {
-    const Cut c = cut_of(g, g.n - at, D, workers);
+    const Cut c = cut_of(g, g.n - at, D, workers, F::WARPS);
+    a.together = c.together;
     a.group = c.group; a.row_tiles = c.row_tiles; a.jobs = c.jobs; a.runs = c.runs; a.slot = c.slot;
     a.prefix = (uint32_t*)scratch;
     a.part = (float*)((char*)scratch + 4096);
@@ -684,13 +771,25 @@ cudaError_t attention_form(const AttnPagesArgs& g, void* scratch, int* launches,
     a.stages = (limit - fixed) / (F::WARPS * F::STAGE);
     if (a.stages > MAX_STAGES) a.stages = MAX_STAGES;
     if (a.stages < 2) return cudaErrorNotSupported;
-    uint64_t blocks = ((uint64_t)c.runs * c.jobs + F::WARPS - 1) / F::WARPS;
+    uint64_t blocks = c.together ? c.n * c.jobs * c.together : ((uint64_t)c.runs * c.jobs + F::WARPS - 1) / F::WARPS;
     if (blocks > (uint64_t)F::BLOCKS * sm_count()) blocks = (uint64_t)F::BLOCKS * sm_count();
-    launch_pdl(attention_pages_kernel<KV, D, QP, EXACT>, dim3((unsigned)blocks), dim3(F::THREADS), fixed + a.stages * F::WARPS * F::STAGE, stream, a);
-    e = cudaGetLastError();
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)blocks); cfg.blockDim = dim3(F::THREADS); cfg.stream = stream;
+    cfg.dynamicSmemBytes = fixed + a.stages * F::WARPS * F::STAGE;
+    cudaLaunchAttribute attr[2];
+    if (pdl_enabled()) {
+      attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+      attr[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
+    }
+    if (c.together > 1) {
+      attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+      attr[cfg.numAttrs].val.clusterDim.x = c.together; attr[cfg.numAttrs].val.clusterDim.y = 1; attr[cfg.numAttrs++].val.clusterDim.z = 1;
+    }
+    cfg.attrs = attr;
+    e = cudaLaunchKernelEx(&cfg, attention_pages_kernel<KV, D, QP, EXACT>, a);
     if (e != cudaSuccess) return e;
     ++*launches;
-    if (c.runs > 1 && c.tiles > 1) {                         // a sequence of one tile is never divided
+    if (!c.together && c.runs > 1 && c.tiles > 1) {                         // a sequence of one tile is never divided
       // a sequence's runs over as many teams as leave each a few (one sequence of 131,001, 148 runs: 105 us by 1,024 threads, 115 by
       // 128; 128 sequences to 8,192, about one run each: 398 by 128, 454 by 1,024)
       constexpr int LANES = D / 4;
@@ -718,27 +817,27 @@ cudaError_t attention_dim(const AttnPagesArgs& g, void* scratch, int* launches, 
 }
 
 template <int D>
-int workers_of(int bf16) {
-  return (bf16 ? Form<uint16_t, D>::BLOCKS * Form<uint16_t, D>::WARPS : Form<float, D>::BLOCKS * Form<float, D>::WARPS) * sm_count();
+size_t scratch_of(const AttnPagesArgs& g) {
+  const int warps = g.cache.bf16 ? Form<uint16_t, D>::WARPS : Form<float, D>::WARPS;
+  const int blocks = g.cache.bf16 ? Form<uint16_t, D>::BLOCKS : Form<float, D>::BLOCKS;
+  const Cut c = cut_of(g, g.n, D, blocks * warps * sm_count(), warps);
+  return c.together ? 0 : 4096 + (size_t)c.runs * c.jobs * 2 * c.slot * sizeof(float);
 }
 
 }  // namespace
 
 bool attention_pages_dim_ok(uint32_t d) { return d == 32 || d == 64 || d == 96 || d == 128 || d == 192 || d == 256; }
 
-// The prefix sums, and two pieces for every (run, head) of the largest launch.
+// The prefix sums, and two pieces for every (run, head) of the largest launch; none where no launch leaves pieces.
 size_t attention_pages_scratch_bytes(const AttnPagesArgs& g) {
-  int workers = 0;
   switch (g.cache.dim) {
-    case 32: workers = workers_of<32>(g.cache.bf16); break;
-    case 64: workers = workers_of<64>(g.cache.bf16); break;
-    case 96: workers = workers_of<96>(g.cache.bf16); break;
-    case 128: workers = workers_of<128>(g.cache.bf16); break;
-    case 192: workers = workers_of<192>(g.cache.bf16); break;
-    default: workers = workers_of<256>(g.cache.bf16); break;
+    case 32: return scratch_of<32>(g);
+    case 64: return scratch_of<64>(g);
+    case 96: return scratch_of<96>(g);
+    case 128: return scratch_of<128>(g);
+    case 192: return scratch_of<192>(g);
+    default: return scratch_of<256>(g);
   }
-  const Cut c = cut_of(g, g.n, (int)g.cache.dim, workers);
-  return 4096 + (size_t)c.runs * c.jobs * 2 * c.slot * sizeof(float);
 }
 
 cudaError_t launch_attention_pages(const AttnPagesArgs& g, void* scratch, int* launches, cudaStream_t stream) {

@@ -312,6 +312,15 @@ def test_attention_long_and_many(eng, lengths, c_bf16, q_bf16):
     attention_case(eng, np.random.default_rng(7), lengths, 4, 2, 64, 16, q_bf16, c_bf16, False)
 
 
+@pytest.mark.parametrize("c_bf16,q_bf16,o_bf16", [(True, True, True), (True, False, False), (False, False, False)])
+@pytest.mark.parametrize("heads,kv,d", [(8, 2, 32), (9, 3, 64), (4, 4, 96), (40, 4, 128), (3, 1, 192), (6, 2, 256)])
+@pytest.mark.parametrize("lengths", [[7], [300], [0], [1, 0, 200], [1000, 3, 0, 17, 16, 999], [129] * 20])
+def test_attention_is_the_same_whatever_the_table_s_width(eng, lengths, heads, kv, d, c_bf16, q_bf16, o_bf16):
+    # A table as wide as the longest needs, and one that leaves room for sequences of 30,000 positions: the work is cut otherwise.
+    for width in (0, 2000):
+        attention_case(eng, np.random.default_rng(len(lengths)), lengths, heads, kv, d, 15, q_bf16, c_bf16, o_bf16, width=width)
+
+
 @pytest.mark.parametrize("window", [1, 2, 15, 16, 17, 64, 100, 699, 700, 701, 100000])
 def test_attention_window(eng, window):
     for c_bf16 in (True, False):
