@@ -248,7 +248,8 @@ __device__ __forceinline__ uint32_t place_of(uint64_t key, const uint64_t* keys,
 // alternatives 2000 BF16 rows of 50257 take 42.6 us (4.7 TB/s) for 44.8 with four, 1000 F32 rows 34.9 (5.8 TB/s) for 39.2; seven
 // blocks a SM leave too few registers (46.8 and 37.3).  Four in the other forms, whose threads have few pieces, and as many
 // blocks as the registers allow (0): more of either costs 16000 rows of 2000 59 -> 70 us and above.
-// Bound by the instructions issued, not by memory: two exponents' and five pairs' operations a pair of values.
+// What bounds the pass is neither limit alone: half of the issue slots and of the exponents' rate, two thirds of a copy's bytes
+// (2000 x 50257 BF16, 25 warps an SM).
 template <typename T, int THREADS, bool SHARED>
 __global__ void __launch_bounds__(THREADS, THREADS == 128 ? 6 : 0) token_logprobs_kernel(const __grid_constant__ LogprobArgs g) {
   constexpr int WARPS = THREADS / 32, N = Vec<T>::N, HELD = THREADS * 8, AHEAD = THREADS == 128 ? 8 : 4;
