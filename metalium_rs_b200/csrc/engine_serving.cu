@@ -287,7 +287,7 @@ int32_t b200_token_logprobs_backward(b200_engine* e, b200_buffer logits, b200_bu
 
 int32_t b200_serving_call(b200_engine* e, int32_t call, uint64_t* w, uint64_t n_words) {
   const uint64_t counts[4] = {19, 17, 16, 12};
-  if (call < 0 || call > 3 || n_words != counts[call])
+  if (call < 0 || call > 3 || !w || n_words != counts[call])
     return e->fail(B200_UNSUPPORTED, "serving_call: call %d of %llu words", call, (ull)n_words);
   const auto f32_of = [](uint64_t word) {
     const uint32_t bits = (uint32_t)word;

@@ -265,6 +265,7 @@ def test_calls_as_words(fake, e):
     send = lambda call, n, *words: fake.b200_serving_call(e._e, C.c_int32(call), w, u64(n)) if not w.__setitem__(slice(0, len(words)), words) else None  # noqa: E731
     for call, n in ((-1, 19), (4, 12), (0, 18), (1, 19), (2, 17), (3, 11)):
         assert send(call, n) == 2
+    assert fake.b200_serving_call(e._e, C.c_int32(0), None, u64(19)) == 2
     c = Cache(e)
     x, p, q = zeros(e, 3, 256, BF16), zeros(e, 1, 3, I32), zeros(e, 3, 128)
     at = C.addressof(c.shape)
