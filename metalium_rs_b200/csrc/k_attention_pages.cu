@@ -19,8 +19,9 @@
 //
 // Precision: keys and values are the cache's own values.  The tensor cores' tile has sixteen rows, and a head takes two of
 // them: row r has an operand's leading part and row r + 8 the next one, so one product does both.  On the BF16 path an F32
-// query is three BF16 parts (exact) or, for a BF16 result, two (2^-16), and so is a probability; on the F32 path every operand
-// is two TF32 parts (2^-22).  For an F32 result a tile's products start from zero and are added to the running rows in F32;
+// query is three BF16 parts (exact, whatever the result's type: a part left out is an error of the score, and a score's error is its
+// weight's relative error however large the score), a probability three or, for a BF16 result, two (2^-16 of it); on the F32
+// path every operand is two TF32 parts (2^-22).  For an F32 result a tile's products start from zero and are added to the running rows in F32;
 // else the tensor cores accumulate them.
 //
 // Measured, heads of 128 (32 over 8), BF16 cache: 128 sequences of 500 to 8,192 393 us = 5.8 TB/s of keys and values (the
@@ -812,7 +813,7 @@ cudaError_t attention_dim(const AttnPagesArgs& g, void* scratch, int* launches, 
   if (!g.cache.bf16) return attention_form<float, D, 2, true>(g, scratch, launches, stream);
   if (g.q.bf16) return g.out_bf16 ? attention_form<uint16_t, D, 1, false>(g, scratch, launches, stream)
                                   : attention_form<uint16_t, D, 1, true>(g, scratch, launches, stream);
-  return g.out_bf16 ? attention_form<uint16_t, D, 2, false>(g, scratch, launches, stream)
+  return g.out_bf16 ? attention_form<uint16_t, D, 3, false>(g, scratch, launches, stream)
                     : attention_form<uint16_t, D, 3, true>(g, scratch, launches, stream);
 }
 
