@@ -19,10 +19,11 @@
 //
 // Precision: keys and values are the cache's own values.  The tensor cores' tile has sixteen rows, and a head takes two of
 // them: row r has an operand's leading part and row r + 8 the next one, so one product does both.  On the BF16 path an F32
-// query is three BF16 parts (exact, whatever the result's type: a part left out is an error of the score, and a score's error is its
-// weight's relative error however large the score), a probability three or, for a BF16 result, two (2^-16 of it); on the F32
-// path every operand is two TF32 parts (2^-22).  For an F32 result a tile's products start from zero and are added to the running rows in F32;
-// else the tensor cores accumulate them.
+// query is three BF16 parts (exact, whatever the result's type: a part left out is an error of the score, and a score's error
+// is its weight's relative error however large the score), a probability three or, for a BF16 result, two (2^-16 of it); on the
+// F32 path every operand is two TF32 parts (2^-22).  A tile's products start from zero and are added to the running rows in
+// F32: the tensor cores cut what they add to a sum, which over the thousands of tiles of a long sequence is a bias (160
+// sequences of 131,072 positions, values of mean 1: 5.7e-4 of the result summed there, 1.5e-6 summed in F32).
 //
 // Measured, heads of 128 (32 over 8), BF16 cache: 128 sequences of 500 to 8,192 393 us = 5.8 TB/s of keys and values (the
 // copies alone, nothing computed, 378), one of 131,001 105 us = 5.1 TB/s (99), 32 of mixed lengths 66 us = 4.1 TB/s (57): what is left
@@ -180,7 +181,6 @@ __device__ __forceinline__ uint32_t sequence_of(const uint32_t* prefix, uint32_t
 template <typename KV, int D, int QP, bool EXACT>
 __global__ void __launch_bounds__(Form<KV, D>::THREADS, Form<KV, D>::BLOCKS) attention_pages_kernel(const __grid_constant__ AttnPlan a) {
   using F = Form<KV, D>;
-  constexpr int ROW_REGS = F::BF && !EXACT ? 4 : 2;       // accumulated by the tensor cores, both parts of a row are
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ uint32_t warp_sum[F::WARPS];
   __shared__ uint32_t valid[F::WARPS][MAX_STAGES];
@@ -352,11 +352,11 @@ __global__ void __launch_bounds__(Form<KV, D>::THREADS, Form<KV, D>::BLOCKS) att
             }
         }
       }
-      float o[D / 8][ROW_REGS];
+      float o[D / 8][2];
 #pragma unroll
       for (int j = 0; j < D / 8; ++j)
 #pragma unroll
-        for (int e = 0; e < ROW_REGS; ++e) o[j][e] = 0.f;
+        for (int e = 0; e < 2; ++e) o[j][e] = 0.f;
       float m = -FLT_MAX, l = 0.f;       // row gr's; the sum is this lane's own
       for (uint32_t step = 0; step < steps; ++step) {
         cp_async_wait(2 * a.stages - 1);
@@ -473,13 +473,6 @@ __global__ void __launch_bounds__(Form<KV, D>::THREADS, Form<KV, D>::BLOCKS) att
             w[1][nt] = bf16x2(u, v);
             if constexpr (EXACT) w[2][nt] = bf16x2(u - low_of(w[1][nt]), v - high_of(w[1][nt]));
           }
-          if constexpr (!EXACT)
-            if (__any_sync(0xffffffffu, f != 1.f)) {
-#pragma unroll
-              for (int j = 0; j < D / 8; ++j)
-#pragma unroll
-                for (int e = 0; e < ROW_REGS; ++e) o[j][e] *= f;
-            }
           const uint32_t vb = v_at + ((lane & 7) + ((lane >> 3) & 1) * 8) * F::V_PITCH + (lane >> 4) * 16;
 #pragma unroll
           for (int j = 0; j < D / 16; ++j) {
@@ -488,15 +481,11 @@ __global__ void __launch_bounds__(Form<KV, D>::THREADS, Form<KV, D>::BLOCKS) att
 #pragma unroll
             for (int hf = 0; hf < 2; ++hf) {
               float* r = o[2 * j + hf];
-              if constexpr (EXACT) {
-                float c[4] = {0.f, 0.f, 0.f, 0.f};
-                mma_bf16(c, 0u, w[2][0], 0u, w[2][1], b[2 * hf], b[2 * hf + 1]);
-                mma_bf16(c, w[0][0], w[1][0], w[0][1], w[1][1], b[2 * hf], b[2 * hf + 1]);
-                r[0] = fmaf(r[0], f, c[0] + c[2]);
-                r[1] = fmaf(r[1], f, c[1] + c[3]);
-              } else {
-                mma_bf16(r, w[0][0], w[1][0], w[0][1], w[1][1], b[2 * hf], b[2 * hf + 1]);
-              }
+              float c[4] = {0.f, 0.f, 0.f, 0.f};
+              if constexpr (EXACT) mma_bf16(c, 0u, w[2][0], 0u, w[2][1], b[2 * hf], b[2 * hf + 1]);
+              mma_bf16(c, w[0][0], w[1][0], w[0][1], w[1][1], b[2 * hf], b[2 * hf + 1]);
+              r[0] = fmaf(r[0], f, c[0] + c[2]);
+              r[1] = fmaf(r[1], f, c[1] + c[3]);
             }
           }
         } else {
@@ -536,9 +525,7 @@ __global__ void __launch_bounds__(Form<KV, D>::THREADS, Form<KV, D>::BLOCKS) att
           const uint64_t at = (uint64_t)here.s * out_cols + (uint64_t)(head0 + gr) * D + 2 * t4;
 #pragma unroll
           for (int j = 0; j < D / 8; ++j) {
-            float u = o[j][0], v = o[j][1];
-            if constexpr (ROW_REGS == 4) { u += o[j][2]; v += o[j][3]; }
-            u /= den; v /= den;
+            const float u = o[j][0] / den, v = o[j][1] / den;
             if (g.out_bf16)
               *reinterpret_cast<uint32_t*>(reinterpret_cast<uint16_t*>(g.out) + at + j * 8) =
                   (uint32_t)f32_to_bf16_bits(__float_as_uint(u)) | ((uint32_t)f32_to_bf16_bits(__float_as_uint(v)) << 16);
@@ -548,11 +535,7 @@ __global__ void __launch_bounds__(Form<KV, D>::THREADS, Form<KV, D>::BLOCKS) att
           // (a warp's own tiles are behind it: their room takes its part where the block joins them)
           float* part = a.together ? reinterpret_cast<float*>(stages) : a.part + ((uint64_t)task * 2 + (piece ? 1 : 0)) * a.slot;
 #pragma unroll
-          for (int j = 0; j < D / 8; ++j) {
-            float u = o[j][0], v = o[j][1];
-            if constexpr (ROW_REGS == 4) { u += o[j][2]; v += o[j][3]; }
-            *reinterpret_cast<float2*>(part + gr * D + j * 8 + 2 * t4) = make_float2(u, v);
-          }
+          for (int j = 0; j < D / 8; ++j) *reinterpret_cast<float2*>(part + gr * D + j * 8 + 2 * t4) = make_float2(o[j][0], o[j][1]);
           if (t4 == 0) *reinterpret_cast<float2*>(part + a.slot / (D + 4) * D + gr * 4) = make_float2(m, l);
         }
       }

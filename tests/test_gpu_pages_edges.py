@@ -1,8 +1,9 @@
-"""`attention_pages` where a result hangs on more than F32's everyday range: large scores.  Definitions in 64 bits; u = 2^-24."""
+"""`attention_pages` where a result hangs on more than F32's everyday range: large scores, sums over thousands of tiles.
+Definitions in 64 bits; u = 2^-24."""
 import numpy as np
 import pytest
 
-from metalium_rs_b200 import PageShape
+from metalium_rs_b200 import BF16, PageShape
 from oracle import oracle as orc
 from tests.test_gpu_pages import U, tables, up, up_i32
 
@@ -45,4 +46,30 @@ def test_large_scores_of_f32_queries(eng, d, o_bf16):
     off = np.abs(got - want)
     assert np.all(off <= tol), float((off / tol).max())
     for i in (iq, ik, iv, it, ip, out):
+        eng.free(i)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_a_long_mean_is_the_nearest_bf16(eng, d):
+    # Zero queries: a result is the mean of about 32,000 values, every other one 2^-9 of the size of its neighbour (512 sequences over
+    # the same pages: every warp sums a run of hundreds of tiles).  Weights and their sum are exact, a sum of sixteen values is within
+    # 4 u; each of T tiles' additions to the running sum rounds to nearest, an error of at most u of it that is as often up as
+    # down: eight standard deviations of T of them are 8 sqrt(T / 3) u, and the division and the joins of a sequence's runs,
+    # 16 at most, are one each.  What remains is the result's own half step.
+    rng = np.random.default_rng(d)
+    n, page, longest = 512, 64, 32768
+    lengths = longest - np.arange(n)
+    ik = eng.zeros_dram((longest, d), BF16)[0]
+    v = rng.uniform(0.5, 1.5, (longest, d)).astype(np.float32)
+    v[1::2] *= np.float32(2.0 ** -9)
+    iv, v = up(eng, v, True)
+    table = np.broadcast_to(np.arange(longest // page, dtype=np.int32), (n, longest // page))
+    it, ip = up_i32(eng, table, *table.shape), up_i32(eng, lengths - 1, 1, n)
+    iq = eng.zeros_dram((n, d), BF16)[0]
+    out, _ = eng.attention_pages(PageShape(1, 1, d, page), (iq, (0, 0), (n, d)), ik, iv, it, ip, 0.125, bf16=True)
+    got = orc.from_bf16(eng.download_bf16(out)).astype(np.float64)
+    want = np.cumsum(v.astype(np.float64), 0)[lengths - 1] / lengths[:, None]
+    tol = (8 * np.sqrt(longest / 16 / 3) + 32) * U * want
+    assert np.all(np.abs(got - want) <= half_step(want) + tol), int((np.abs(got - want) > half_step(want) + tol).sum())
+    for i in (ik, iv, it, ip, iq, out):
         eng.free(i)
