@@ -521,7 +521,8 @@ __global__ void __launch_bounds__(Form<KV, D>::THREADS, Form<KV, D>::BLOCKS) att
       l += __shfl_xor_sync(0xffffffffu, l, 2);
       if (gr < (int)rows) {
         if (whole && !a.together) {
-          const float den = l < FLT_MIN ? FLT_MIN : l;
+          // an infinite largest score: the differences to it leave no weight, where the steps' exp(inf - inf) is NaN
+          const float den = m == INFINITY ? NAN : (l < FLT_MIN ? FLT_MIN : l);
           const uint64_t at = (uint64_t)here.s * out_cols + (uint64_t)(head0 + gr) * D + 2 * t4;
 #pragma unroll
           for (int j = 0; j < D / 8; ++j) {

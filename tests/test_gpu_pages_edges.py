@@ -1,9 +1,9 @@
-"""`attention_pages` where a result hangs on more than F32's everyday range: large scores, sums over thousands of tiles.
-Definitions in 64 bits; u = 2^-24."""
+"""`attention_pages` where a result hangs on more than F32's everyday range: large scores, sums over thousands of tiles, scores
+that leave the type's range.  Definitions in 64 bits; u = 2^-24."""
 import numpy as np
 import pytest
 
-from metalium_rs_b200 import BF16, PageShape
+from metalium_rs_b200 import BF16, BOOL, PageShape
 from oracle import oracle as orc
 from tests.test_gpu_pages import U, tables, up, up_i32
 
@@ -72,4 +72,59 @@ def test_a_long_mean_is_the_nearest_bf16(eng, d):
     tol = (8 * np.sqrt(longest / 16 / 3) + 32) * U * want
     assert np.all(np.abs(got - want) <= half_step(want) + tol), int((np.abs(got - want) > half_step(want) + tol).sum())
     for i in (ik, iv, it, ip, iq, out):
+        eng.free(i)
+
+
+def rows_and_pages(eng, q, k, v, scale, c_bf16, o_bf16, width):
+    """The result of `attention_rows` and of `attention_pages`, [heads, d], for one sequence of whole positions, one key/value head."""
+    heads, d = q.shape
+    n, page = len(k), 16
+    iq, ik, iv = up(eng, q, False)[0], up(eng, k, c_bf16)[0], up(eng, v, c_bf16)[0]
+    mask = eng.upload_bits(np.zeros((1, n), np.uint32), 1, n, BOOL)
+    one, _ = eng.attention_rows((iq, ik, iv, mask), [((h, 0), (0, 0), (0, 0)) for h in range(heads)], (1, d, n, d), scale)
+    table = np.zeros((1, max(n // page, width)), np.int32)
+    table[0, :n // page] = np.arange(n // page)
+    it, ip = up_i32(eng, table, *table.shape), up_i32(eng, [n - 1], 1, 1)
+    flat, _ = eng.reshape(iq, 1, heads * d)
+    two, _ = eng.attention_pages(PageShape(heads, 1, d, page), (flat, (0, 0), (1, heads * d)), ik, iv, it, ip, scale, bf16=o_bf16)
+    a = eng.download(one).reshape(heads, d)
+    b = (orc.from_bf16(eng.download_bf16(two)) if o_bf16 else eng.download(two)).reshape(heads, d)
+    for i in (iq, ik, iv, mask, one, it, ip, flat, two):
+        eng.free(i)
+    return a, b
+
+
+@pytest.mark.parametrize("c_bf16,o_bf16", [(True, False), (True, True), (False, False)])
+@pytest.mark.parametrize("width", [0, 3000])
+@pytest.mark.parametrize("n", [32, 320])
+def test_a_score_beyond_the_type_s_range(eng, n, width, c_bf16, o_bf16):
+    # A product of 1e30 times a scale of 1e10 is infinite in F32: NaN, as the composition's steps give; to -inf it is weight 0.
+    rng = np.random.default_rng(n)
+    q, k = np.zeros((2, 64), np.float32), rng.standard_normal((n, 64)).astype(np.float32) * np.float32(1e-10)
+    q[:, 0], q[:, 1], k[:, 0] = [2.0 ** 50, -2.0 ** 50], 1.0, 0.0
+    k[n - 3, 0] = 2.0 ** 50
+    v = rng.standard_normal((n, 64)).astype(np.float32)
+    a, b = rows_and_pages(eng, q, k, v, 1e10, c_bf16, o_bf16, width)
+    assert np.isnan(a[0]).all() and np.isfinite(a[1]).all()
+    assert np.isnan(b[0]).all()
+    # scores within 4, weights by (64 + 24) u of them and of their functions; the result's own step
+    assert np.all(np.abs(a[1] - b[1]) <= 4 * 88 * 8 * U * np.abs(v).max() + (2.0 ** -8 if o_bf16 else U) * np.abs(a[1]))
+
+
+@pytest.mark.parametrize("c_bf16", [True, False])
+@pytest.mark.parametrize("length", [16, 40])
+def test_a_score_beyond_the_type_s_range_at_a_sequence_s_end(eng, length, c_bf16):
+    # The same for sequences that one warp sums whole, the infinite score the last of its last tile.
+    rng = np.random.default_rng(length)
+    n, page = 600, 16
+    table, pages = tables(rng, [length] * n, page)
+    q, k = np.ones((n, 64), np.float32), rng.standard_normal((pages * page, 64)).astype(np.float32) * np.float32(1e-12)
+    q[:, 0], k[:, 0] = 2.0 ** 50, 0.0
+    k[table[:, (length - 1) // page] * page + (length - 1) % page, 0] = 2.0 ** 50
+    iq, ik = up(eng, q, False)[0], up(eng, k, c_bf16)[0]
+    iv = up(eng, rng.standard_normal((pages * page, 64)).astype(np.float32), c_bf16)[0]
+    it, ip = up_i32(eng, table, *table.shape), up_i32(eng, np.full(n, length - 1), 1, n)
+    out, _ = eng.attention_pages(PageShape(1, 1, 64, page), (iq, (0, 0), (n, 64)), ik, iv, it, ip, 1e10)
+    assert np.isnan(eng.download(out)).all()
+    for i in (iq, ik, iv, it, ip, out):
         eng.free(i)
