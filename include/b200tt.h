@@ -479,8 +479,9 @@ int32_t b200_rope_append_pages(b200_engine*, const b200_page_shape* shape, const
  * the cache already; query head h reads key/value head h / (heads / kv_heads).  It attends to positions 0 .. positions[i], or
  * with window > 0 to the last `window` of them.  out [n, heads * head_dim] = softmax(scale q K^T) V with `attention_rows`'
  * steps in F32 (clamped maximum and sum: a row that attends to nothing, positions[i] == -1 or scores all -inf, is zero),
- * rounded once with out_bf16.  Nothing behind a sequence's last position is read.  An infinite or NaN value at an attended
- * position makes its column NaN (infinite keys give what their scores are); F32 values are below 3.4e38 in magnitude.
+ * rounded once with out_bf16.  Nothing behind a sequence's last position is read.  Infinite and NaN keys
+ * and values at attended positions give what those steps make of them; weighted sums are taken before the division and stay
+ * within F32's range.
  * Refused unless head_dim is 32, 64, 96, 128, 192 or 256, heads is a multiple of kv_heads and scale lies within
  * -1e20 .. 1e20. */
 int32_t b200_attention_pages(b200_engine*, const b200_page_shape* shape, const b200_block_arg* q, b200_buffer key_pages,

@@ -177,6 +177,47 @@ __device__ __forceinline__ uint32_t sequence_of(const uint32_t* prefix, uint32_t
   return lo;
 }
 
+// A part [rows][D], or with no `part` the result's rows, again from whole operands: where a value is infinite (or an F32 one too
+// large for its parts) the products of the parts hold 0 * inf, which the steps do not.  `top` and `den` are row lane / 4's.  A lane a
+// position for the scores, a lane every 32nd column for the rows: rare, so it is simple and out of the way.
+template <typename KV, int D>
+__device__ __noinline__ void sum_again(const AttnPlan& a, uint32_t s, uint32_t first, uint32_t end, uint32_t kvh, uint32_t head0, uint32_t rows,
+                                       float tops, float dens, float* part) {
+  const AttnPagesArgs& g = a.g;
+  const uint32_t lane = threadIdx.x % 32;
+  const uint64_t ld = (uint64_t)g.cache.kv_heads * D, head_at = (uint64_t)kvh * D;
+  for (uint32_t r = 0; r < rows; ++r) {
+    const float top = __shfl_sync(0xffffffffu, tops, r * 4), den = __shfl_sync(0xffffffffu, dens, r * 4);
+    float v[D / 32];
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) v[i] = 0.f;
+    for (uint32_t p0 = first; p0 < end; p0 += 32) {
+      const int64_t row = p0 + lane < end ? pool_row(g.cache, s, p0 + lane, g.err) : -1;
+      float w = 0.f;
+      if (row >= 0) {
+        for (int i = 0; i < D; ++i)
+          w = fmaf(load_float(g.q.p, (uint64_t)s * g.q.ld + (uint64_t)(head0 + r) * D + i, g.q.bf16),
+                   load_float(g.cache.keys, (uint64_t)row * ld + head_at + i, sizeof(KV) == 2), w);
+        w = exp2_fast(fmaf(w, a.scale_log2, -top));
+        w = w > 1.f ? 1.f : w;           // summed in another order than `top`'s, a score may lie a rounding above it
+      }
+      for (int j = 0; j < 32; ++j) {
+        const int64_t from = __shfl_sync(0xffffffffu, row, j);
+        const float x = __shfl_sync(0xffffffffu, w, j);
+        if (from >= 0)
+#pragma unroll
+          for (int i = 0; i < D / 32; ++i)
+            v[i] = fmaf(x, load_float(g.cache.values, (uint64_t)from * ld + head_at + i * 32 + lane, sizeof(KV) == 2), v[i]);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) {
+      if (part) part[r * D + i * 32 + lane] = v[i];
+      else store_float(g.out, ((uint64_t)s * g.cache.heads + head0 + r) * D + i * 32 + lane, g.out_bf16, v[i] / den);
+    }
+  }
+}
+
 // QP: the queries' parts.  EXACT: an F32 result.
 template <typename KV, int D, int QP, bool EXACT>
 __global__ void __launch_bounds__(Form<KV, D>::THREADS, Form<KV, D>::BLOCKS) attention_pages_kernel(const __grid_constant__ AttnPlan a) {
@@ -519,10 +560,14 @@ __global__ void __launch_bounds__(Form<KV, D>::THREADS, Form<KV, D>::BLOCKS) att
       // ---- the sequence's result, or its part of one
       l += __shfl_xor_sync(0xffffffffu, l, 1);
       l += __shfl_xor_sync(0xffffffffu, l, 2);
+      // an infinite largest score: the differences to it leave no weight, where the steps' exp(inf - inf) is NaN
+      const float den = m == INFINITY ? NAN : (l < FLT_MIN ? FLT_MIN : l);
+      float* part = nullptr;             // (a warp's own tiles are behind it: their room takes its part where the block joins them)
+      if (a.together) part = reinterpret_cast<float*>(stages);
+      else if (!whole) part = a.part + ((uint64_t)task * 2 + (piece ? 1 : 0)) * a.slot;
+      float odd = 0.f;                   // NaN where a sum is no finite number
       if (gr < (int)rows) {
-        if (whole && !a.together) {
-          // an infinite largest score: the differences to it leave no weight, where the steps' exp(inf - inf) is NaN
-          const float den = m == INFINITY ? NAN : (l < FLT_MIN ? FLT_MIN : l);
+        if (!part) {
           const uint64_t at = (uint64_t)here.s * out_cols + (uint64_t)(head0 + gr) * D + 2 * t4;
 #pragma unroll
           for (int j = 0; j < D / 8; ++j) {
@@ -533,12 +578,17 @@ __global__ void __launch_bounds__(Form<KV, D>::THREADS, Form<KV, D>::BLOCKS) att
             else *reinterpret_cast<float2*>(reinterpret_cast<float*>(g.out) + at + j * 8) = make_float2(u, v);
           }
         } else {
-          // (a warp's own tiles are behind it: their room takes its part where the block joins them)
-          float* part = a.together ? reinterpret_cast<float*>(stages) : a.part + ((uint64_t)task * 2 + (piece ? 1 : 0)) * a.slot;
 #pragma unroll
           for (int j = 0; j < D / 8; ++j) *reinterpret_cast<float2*>(part + gr * D + j * 8 + 2 * t4) = make_float2(o[j][0], o[j][1]);
           if (t4 == 0) *reinterpret_cast<float2*>(part + a.slot / (D + 4) * D + gr * 4) = make_float2(m, l);
         }
+#pragma unroll
+        for (int j = 0; j < D / 8; ++j) odd = fmaf(o[j][0], 0.f, fmaf(o[j][1], 0.f, odd));
+      }
+      if (__any_sync(0xffffffffu, odd != odd)) {
+        __syncwarp();                    // what the lanes have written is written again by others
+        const uint32_t first = here.lo + here.tile * 16, end = min(here.end, first + steps * 16);
+        sum_again<KV, D>(a, here.s, first, end, kvh, head0, rows, m, den, part);
       }
       left -= steps;
       here.tile += steps;

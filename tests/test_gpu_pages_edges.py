@@ -1,5 +1,5 @@
 """`attention_pages` where a result hangs on more than F32's everyday range: large scores, sums over thousands of tiles, scores
-that leave the type's range.  Definitions in 64 bits; u = 2^-24."""
+that leave the type's range, infinities and NaN among the attended values.  Definitions in 64 bits; u = 2^-24."""
 import numpy as np
 import pytest
 
@@ -128,3 +128,46 @@ def test_a_score_beyond_the_type_s_range_at_a_sequence_s_end(eng, length, c_bf16
     assert np.isnan(eng.download(out)).all()
     for i in (iq, ik, iv, it, ip, out):
         eng.free(i)
+
+
+@pytest.mark.parametrize("c_bf16,o_bf16", [(True, False), (True, True), (False, False)])
+@pytest.mark.parametrize("heads,d", [(1, 32), (8, 64), (3, 96), (11, 128), (2, 192), (4, 256)])
+@pytest.mark.parametrize("n,width", [(32, 0), (320, 0), (320, 3000), (4096, 0)])
+def test_infinite_and_nan_values(eng, n, width, heads, d, c_bf16, o_bf16):
+    # What the composition's steps make of values that are no numbers: an infinity stays one, +inf beside -inf and a NaN are NaN,
+    # and so is an infinity whose weight is 0.  The other columns are as if there were none.
+    rng = np.random.default_rng(n + d)
+    q, k, v = ((rng.standard_normal(s) * f).astype(np.float32) for s, f in (((heads, d), 0.3), ((n, d), 0.3), ((n, d), 1.0)))
+    k = orc.from_bf16(orc.to_bf16(k)) if c_bf16 else k
+    v = orc.from_bf16(orc.to_bf16(v)) if c_bf16 else v
+    v[3, 0], v[n - 1, 1], v[n // 2, 5] = np.inf, -np.inf, np.nan
+    v[5, 9], v[n - 2, 9] = np.inf, -np.inf                      # both in one column
+    v[16, 11], v[17, 11] = np.inf, np.inf
+    v[n // 2, 30] = np.inf
+    if not c_bf16:
+        v[9, 13] = np.finfo(np.float32).max                     # the largest value is one like the others
+    a, b = rows_and_pages(eng, q, k, v, 0.5, c_bf16, o_bf16, width)
+    assert np.isposinf(a[:, [0, 11, 30]]).all() and np.isneginf(a[:, 1]).all() and np.isnan(a[:, [5, 9]]).all()
+    assert np.array_equal(np.isnan(a), np.isnan(b)) and np.array_equal(np.isinf(a), np.isinf(b))
+    fin = np.isfinite(a)
+    assert np.array_equal(np.sign(a[~fin]), np.sign(b[~fin]), equal_nan=True)
+    # each form's scores: (d + 24) u of sum |q k|, and 2^-21 of it for operands in parts; its weights by that, numerator and
+    # denominator; the sums n / 16 + 32 roundings; a weight's own parts; the result's step
+    size = np.broadcast_to(np.where(np.isfinite(v), np.abs(v), 0).max(0), a.shape)
+    mass = float((np.abs(q) @ np.abs(k).T).max()) * 0.5
+    tol = (4 * ((d + 24) * U + 2.0 ** -21) * (mass + 1) + 4 * (n / 16 + 32) * U + (2.0 ** -16 if o_bf16 else 2.0 ** -20)) * size
+    tol = tol + (2.0 ** -8 if o_bf16 else U) * (np.abs(a) + tol)
+    with np.errstate(invalid="ignore"):
+        assert np.all((np.abs(a - b) <= tol)[fin])
+
+
+def test_an_infinite_value_behind_a_weight_of_zero(eng):
+    # its product is NaN; behind the sequence's last position, or before its window, it is not read
+    rng = np.random.default_rng(5)
+    q, k, v = (rng.standard_normal(s).astype(np.float32) for s in ((2, 64), (64, 64), (64, 64)))
+    q[:, 4] = 1.0
+    k[10, 4] = -np.inf
+    v[10, 2] = np.inf
+    for c_bf16 in (True, False):
+        a, b = rows_and_pages(eng, q, k, v, 0.25, c_bf16, False, 0)
+        assert np.isnan(a[:, 2]).all() and np.array_equal(np.isnan(a), np.isnan(b))
