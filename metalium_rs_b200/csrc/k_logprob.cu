@@ -3,7 +3,8 @@
 //
 // With y = scale x, m = max y, S = sum e^(y - m) and T = sum e^(y - m) (y - m):
 //   lse = m + log S,   log p_j = (y_j - m) - log S,   entropy = log S - T / S.
-// Both terms of the entropy are of one sign (T <= 0), so nothing cancels.  Values are ordered as `argmax_row` orders them
+// Both terms of the entropy are of one sign (T <= 0; m is rounded, so to its last bit), and for a row sure of one token log S is
+// as small as that token's log probability: nothing cancels.  Values are ordered as `argmax_row` orders them
 // (a NaN above everything, -0 equal to +0, equal values by the lower column): one 64-bit key a value.
 #include <cfloat>
 #include <cmath>
@@ -165,20 +166,27 @@ template <typename T, int THREADS> struct Slice {
   }
 };
 
+// The largest of a warp's values, NaN passed over.
+__device__ __forceinline__ float warp_max(float v) {
+  float r;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
+}
+
 // A thread's running state over its pieces: its largest value and the first piece that has it, the largest of the others, and
-// the sums.  The reference
-// follows the largest value only when that is 2^16 above it: within that, terms and sums keep their bits, and the step that
-// moves it (a thread meets four new maxima in 25 pieces, so one of a warp's threads meets one in almost every piece) stays rare.
+// the sums under the reference m = fl(high c).  `high` is the largest value that the warp had met when it last asked (at least
+// LOW, and with nothing above that the thread has no reference), and the warp asks before it sums: a reference that stayed
+// behind the largest term by z would leave the entropy and a sure token's log probability as differences of two numbers near z.
 template <typename T> struct Running {
-  float best = -INFINITY, second = -INFINITY, m = 0.f;
+  float best = -INFINITY, second = -INFINITY, high = LOW, m = 0.f;
   uint32_t piece;
   uint64_t s[2] = {0, 0}, t[2] = {0, 0};
-  __device__ __forceinline__ void take(const uint4& w, uint32_t u, float c, uint64_t c2) {
-    const float top = Vec<T>::top(w), at = fmaf(top, c, -m);
-    if (at > 16.f || (best <= LOW && top > LOW)) move(fminf(fmaxf(top * c, -FLT_MAX), FLT_MAX));
+  __device__ __forceinline__ void note(float top, uint32_t u) {
     piece = top > best ? u : piece;
     second = fmaxf(second, fminf(top, best));
     best = fmaxf(best, top);
+  }
+  __device__ __forceinline__ void add(const uint4& w, uint64_t c2) {
     uint64_t v[Vec<T>::N / 2];
     Vec<T>::pairs(w, v);
     const uint64_t ref = pair_of(-m, -m);
@@ -193,13 +201,21 @@ template <typename T> struct Running {
   }
   __device__ __forceinline__ Sums sums() const {           // a thread with nothing above LOW has no reference
     const float2 a = floats_of(add2(s[0], s[1])), b = floats_of(add2(t[0], t[1]));
-    return Sums{best > LOW ? m : -FLT_MAX, a.x + a.y, b.x + b.y};
+    return Sums{high > LOW ? m : -FLT_MAX, a.x + a.y, b.x + b.y};
   }
-  __device__ __forceinline__ void move(float to) {
-    const Sums a = under(Sums{m, sums().s, sums().t}, to);
+  __device__ __forceinline__ void raise(float to, float c) {
+    if (!(to > high)) return;
+    high = to;
+    const Sums a = under(Sums{m, sums().s, sums().t}, fminf(fmaxf(to * c, -FLT_MAX), FLT_MAX));
     s[0] = pair_of(a.s, 0.f); t[0] = pair_of(a.t, 0.f);
     s[1] = t[1] = 0;
-    m = to;
+    m = a.m;
+  }
+  __device__ __forceinline__ void alone(const uint4& w, uint32_t u, float c, uint64_t c2) {   // a piece of this thread only
+    const float top = Vec<T>::top(w);
+    raise(top, c);
+    note(top, u);
+    add(w, c2);
   }
 };
 
@@ -244,15 +260,16 @@ __device__ __forceinline__ uint32_t place_of(uint64_t key, const uint64_t* keys,
 // thread's read by the block.  What reaches the bound is listed and put in order.  Where that is more than the list holds -- rows
 // of few distinct values -- the bound is taken again from keys, by value and column.
 //
-// A thread asks for AHEAD of its pieces before it uses the first.  Eight where rows are long, with six blocks a SM: without
-// alternatives 2000 BF16 rows of 50257 take 42.6 us (4.7 TB/s) for 44.8 with four, 1000 F32 rows 34.9 (5.8 TB/s) for 39.2; seven
-// blocks a SM leave too few registers (46.8 and 37.3).  Four in the other forms, whose threads have few pieces, and as many
-// blocks as the registers allow (0): more of either costs 16000 rows of 2000 59 -> 70 us and above.
+// A thread asks for AHEAD of its pieces before it uses the first, and a warp for its largest value every ASKED of them.  Eight and
+// four where rows are long, with the registers of seven blocks an SM: without alternatives 2000 BF16 rows of 50257 take 44.1 us
+// (4.6 TB/s), 1000 F32 rows 34.9 (5.8 TB/s); asking every two 43.8 and 34.9, every eight 46.4 and 36.4; with six blocks' registers
+// 47.0 and 45.1 (1000 rows are more than one round of blocks then).  Four pieces in the other forms, whose threads have few, and as
+// many blocks as the registers allow (0): more of either costs 16000 rows of 2000 59 -> 70 us and above.
 // What bounds the pass is neither limit alone: half of the issue slots and of the exponents' rate, two thirds of a copy's bytes
-// (2000 x 50257 BF16, 25 warps an SM).
+// (2000 x 50257 BF16, 28 warps an SM).
 template <typename T, int THREADS, bool SHARED>
-__global__ void __launch_bounds__(THREADS, THREADS == 128 ? 6 : 0) token_logprobs_kernel(const __grid_constant__ LogprobArgs g) {
-  constexpr int WARPS = THREADS / 32, N = Vec<T>::N, HELD = THREADS * 8, AHEAD = THREADS == 128 ? 8 : 4;
+__global__ void __launch_bounds__(THREADS, THREADS == 128 ? 7 : 0) token_logprobs_kernel(const __grid_constant__ LogprobArgs g) {
+  constexpr int WARPS = THREADS / 32, N = Vec<T>::N, HELD = THREADS * 8, AHEAD = THREADS == 128 ? 8 : 4, ASKED = 4;
   __shared__ uint64_t held[HELD], sh[WARPS], slices[SHARED ? CLUSTER * TOP : TOP], list[TOP];
   __shared__ Sums warp_sums[WARPS], slice_sums[SHARED ? CLUSTER : 1];
   __shared__ float warp_best[WARPS], slice_best[SHARED ? CLUSTER : 1];
@@ -284,17 +301,35 @@ __global__ void __launch_bounds__(THREADS, THREADS == 128 ? 6 : 0) token_logprob
   Running<T> a;
   a.piece = (uint32_t)tid;               // a thread whose values are all -inf has its first
   const uint32_t lo = sl.pieces && !sl.whole(0) ? 1u : 0u, hi = sl.pieces && !sl.whole(sl.pieces - 1) ? sl.pieces - 1 : sl.pieces;
-  if (lo && tid == 0) a.take(sl.piece(0), 0, c, c2);
-  for (uint32_t u = lo && tid == 0 ? THREADS : tid; u < hi; u += AHEAD * THREADS) {
+  if (lo && tid == 0) a.alone(sl.piece(0), 0, c, c2);
+  const uint32_t gone = sizeof(T) == 2 ? 0xff80ff80u : 0xff800000u;           // a lane without a piece: -inf
+  for (uint32_t u = tid; u - lane < hi; u += AHEAD * THREADS) {               // the same for a warp's lanes
     uint4 w[AHEAD];
 #pragma unroll
-    for (int i = 0; i < AHEAD; ++i)
-      if (u + i * THREADS < hi) w[i] = sl.raw(u + i * THREADS);
+    for (int i = 0; i < AHEAD; ++i) {
+      const uint32_t v = u + i * THREADS;
+      w[i] = make_uint4(gone, gone, gone, gone);
+      if (v >= lo && v < hi) w[i] = sl.raw(v);
+    }
 #pragma unroll
-    for (int i = 0; i < AHEAD; ++i)
-      if (u + i * THREADS < hi) a.take(w[i], u + i * THREADS, c, c2);
+    for (int k = 0; k < AHEAD; k += ASKED) {
+      if (u - lane + k * THREADS >= hi) break;
+      float tops[ASKED], most = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < ASKED; ++i) {
+        tops[i] = Vec<T>::top(w[k + i]);
+        most = fmaxf(most, tops[i]);
+      }
+      if (__any_sync(0xffffffffu, most > a.high)) a.raise(warp_max(most), c);
+#pragma unroll
+      for (int i = 0; i < ASKED; ++i)
+        if (u - lane + (k + i) * THREADS < hi) {
+          a.note(tops[i], u + (k + i) * THREADS);
+          a.add(w[k + i], c2);
+        }
+    }
   }
-  if (hi < sl.pieces && hi >= lo && sl.pieces > lo && tid == (int)(hi % THREADS)) a.take(sl.piece(hi), hi, c, c2);
+  if (hi < sl.pieces && hi >= lo && sl.pieces > lo && tid == (int)(hi % THREADS)) a.alone(sl.piece(hi), hi, c, c2);
 
   // ---- the slice's sums: under the largest reference of the warp, then of the block
   Sums all = a.sums();
