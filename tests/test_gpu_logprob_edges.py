@@ -1,11 +1,81 @@
-"""`token_logprobs` on rows where the everyday tolerance shows nothing: rows sure of one token.  Definitions in 64 bits; u = 2^-24."""
+"""`token_logprobs` on rows where the everyday tolerance shows nothing: rows sure of one token, rows masked by the type's lowest
+values, rows far from zero.  Definitions in 64 bits; u = 2^-24.
+
+What a row's results are held to goes by the terms that carry weight: with m the row's largest y, a term e^(y - m) is within
+6 u |y - m| + 8 u of itself, which weighted by the term is below 12 u; the additions of a row of up to 32,768 are within 512 u;
+so log sum, entropy (another factor |y - m|, weighted) and a log probability are within 600 u (1 + |entropy|) and 6 u |y - m| of the
+token's own, whatever |m|, and only lse, which holds m itself, by 4 u |m| more."""
 import numpy as np
 import pytest
 
 from oracle import oracle as orc
-from tests.test_gpu_logprobs import U, run
+from tests.test_gpu_logprobs import U, logits, run
 
 pytestmark = pytest.mark.gpu
+
+
+def weighted(eng, x, ids, scale=1.0, top=0, bf16=False):
+    x, got = run(eng, x, ids, scale, top, bf16)
+    n, cols = x.shape
+    y = x.astype(np.float64) * np.float64(np.float32(scale))
+    m = y.max(1)
+    z = y - m[:, None]
+    p = np.exp(z)
+    s = p.sum(1)
+    p /= s[:, None]
+    log = z - np.log(s)[:, None]
+    ent = -np.where(p > 0, p * log, 0).sum(1)
+    spread = np.where(p > 0, p * -z, 0).sum(1)
+    sums = 600 * U * (1 + ent + spread)
+    r = np.arange(n)
+    token = np.where(ids < 0, 0.0, log[r, np.maximum(ids, 0)])
+    own = np.where(ids < 0, 0.0, -z[r, np.maximum(ids, 0)])
+    assert np.all(np.abs(got[0] - token) <= sums + 6 * U * own), (got[0], token)
+    assert np.all(np.abs(got[1] - ent) <= sums), (got[1], ent)
+    assert np.all(np.abs(got[2] - (m + np.log(s))) <= sums + 4 * U * np.abs(m)), (got[2], m + np.log(s))
+    if top:
+        best = np.argsort(-x.astype(np.float64), 1, kind="stable")[:, :top]
+        assert np.array_equal(got[3], best)
+        assert np.all(np.abs(got[4] - np.take_along_axis(log, best, 1)) <= sums[:, None] + 6 * U * -np.take_along_axis(z, best, 1))
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("rows,cols", [(9, 40), (9, 1000), (9, 3001), (300, 3001), (300, 20011), (9, 32768)])
+def test_rows_masked_by_the_type_s_lowest_values(eng, rows, cols, bf16):
+    rng = np.random.default_rng(cols)
+    x = logits(rng, rows, cols)
+    low = orc.from_bf16(np.array([0xFF7F], np.uint16))[0] if bf16 else np.finfo(np.float32).min
+    for i, mask in enumerate((-3.0e38, low, -1.0e30, -1.0e31, -2.0e9)):
+        live = rng.random(cols) < 0.2
+        live[cols // 2] = True
+        x[i] = np.where(live, x[i], mask)
+    x[5], x[6], x[7] = low, -1.0e30, -1.0e31                # nothing left: all alike
+    x[8], x[8, 1] = -3.0e38, -2.9e38
+    ids = np.full(rows, cols // 2)
+    for top in (0, min(20, cols)):
+        weighted(eng, x, ids, 1.0, top, bf16)
+
+
+@pytest.mark.parametrize("rows,cols", [(8, 100), (8, 3000), (300, 3000), (300, 12000), (2, 32768)])
+def test_rows_far_from_zero_keep_their_differences(eng, rows, cols):
+    # In 1e8 .. 4e8, where F32's step is 8 to 32, and beyond: three largest and ten next to them, the others far below.
+    rng = np.random.default_rng(rows + cols)
+    base = np.array([1.0e6, -1.0e6, 1.2e8, -1.2e8, 4.0e8, 3.0e12, -3.0e12, 2.0e30])
+    x = np.empty((rows, cols), np.float32)
+    scale = 0.25
+    for i in range(rows):
+        b = np.float32(base[i % len(base)])
+        step = np.spacing(np.abs(b))
+        at = rng.permutation(cols)
+        x[i] = b - 4000 * step
+        x[i, at[:3]] = b
+        x[i, at[3:13]] = b - step
+        x[i, at[13:30]] = b - 2 * step
+    ids = x.argmax(1)
+    ids[1::2] = [int(np.flatnonzero(r == r.max() - np.spacing(np.abs(r.max())))[0]) if (r == r.max() - np.spacing(np.abs(r.max()))).any() else 0
+                 for r in x[1::2]]
+    weighted(eng, x, ids, scale, 5)
+    weighted(eng, x, ids, 1.0)
 
 
 @pytest.mark.parametrize("bf16", [False, True])
