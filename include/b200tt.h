@@ -505,8 +505,8 @@ int32_t b200_token_logprobs(b200_engine*, b200_buffer logits, b200_buffer ids, f
  * d_logprob and d_entropy (F32, rows values; d_entropy and entropy 0: absent),
  *   out = scale * (d_logprob (1[column = id] - p) - d_entropy p (y - lse + entropy)),
  * F32 or rounded once to BF16, [rows, vocab].  lse and entropy are the forward's.  A row whose id is -1 has no d_logprob
- * term; an entry of -inf has gradient 0 (its own 1[column = id] term apart), a row of -inf only is zero.  Refused as the
- * forward is. */
+ * term, and is zero whatever its logits hold where d_entropy is absent or 0 too; an entry of -inf has gradient 0 (its own
+ * 1[column = id] term apart), a row of -inf only is zero.  Refused as the forward is. */
 int32_t b200_token_logprobs_backward(b200_engine*, b200_buffer logits, b200_buffer ids, b200_buffer lse, b200_buffer entropy,
                                      b200_buffer d_logprob, b200_buffer d_entropy, float scale, int32_t out_bf16,
                                      b200_buffer into, b200_buffer* out, uint64_t out_dims[2]);

@@ -585,7 +585,8 @@ __global__ void __launch_bounds__(256) token_logprobs_backward_kernel(const __gr
   if (!named && id != -1 && threadIdx.x == 0) atomicCAS(g.err, 0, DOMAIN_ERROR);
   const float up = named ? given : 0.f;
   const uint32_t hot = named ? (uint32_t)id : 0xffffffffu;
-  const bool empty = lse == -INFINITY;
+  // a row of -inf only, and a row with neither gradient (a padding row, whatever its logits hold: 0 * NaN is NaN)
+  const bool empty = lse == -INFINITY || (!named && (!ENTROPY || h == 0.f));
   const float flat = ENTROPY ? fmaf(h, H, -up) : -up;
   // p (h (z + H) - up), z = y - lse; with a z below -1000, where p is 0, its factor stays finite
   const auto value = [&](uint64_t v, float& v0, float& v1) {
@@ -605,7 +606,7 @@ __global__ void __launch_bounds__(256) token_logprobs_backward_kernel(const __gr
       float v[8];
 #pragma unroll
       for (int e = 0; e < 4; ++e) value(x[i][e], v[2 * e], v[2 * e + 1]);
-      if (hot - col < 8 || empty)                            // the given token's own term, and a row of -inf only
+      if (hot - col < 8 || empty)                            // the given token's own term, and an empty row
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = empty ? 0.f : (col + e == hot ? v[e] + up : v[e]);
       if constexpr (OUT_BF) {

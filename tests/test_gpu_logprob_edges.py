@@ -1,5 +1,5 @@
-"""`token_logprobs` on rows where the everyday tolerance shows nothing: rows sure of one token, rows masked by the type's lowest
-values, rows far from zero.  Definitions in 64 bits; u = 2^-24.
+"""`token_logprobs` and its gradient on rows where the everyday tolerance shows nothing: rows sure of one token, rows masked by the
+type's lowest values, rows far from zero, padding rows.  Definitions in 64 bits; u = 2^-24.
 
 What a row's results are held to goes by the terms that carry weight: with m the row's largest y, a term e^(y - m) is within
 6 u |y - m| + 8 u of itself, which weighted by the term is below 12 u; the additions of a row of up to 32,768 are within 512 u;
@@ -9,7 +9,7 @@ import numpy as np
 import pytest
 
 from oracle import oracle as orc
-from tests.test_gpu_logprobs import U, logits, run
+from tests.test_gpu_logprobs import U, grad64, logits, run, up, up_i32
 
 pytestmark = pytest.mark.gpu
 
@@ -99,3 +99,38 @@ def test_rows_sure_of_one_token(eng, rows, cols, apart, bf16):
     assert np.all(np.abs(got[1] - ent) <= 12 * U), float(np.abs(got[1] - ent).max() / U)
     assert np.all(np.abs(got[4][:, 0] - log) <= 8 * U)
     assert np.all(got[0] <= 0) and np.all(got[1] >= 0)
+
+
+# ------------------------------------------------------------------------------------------------ the gradient
+def gradient(eng, x, ids, g, h, scale, bf16, o_bf16):
+    n, cols = x.shape
+    ix, x = up(eng, x, bf16)
+    ii = up_i32(eng, ids, n, 1)
+    (lp, _), (en, _), (ls, _) = eng.token_logprobs(ix, ii, scale)
+    ig = eng.upload(g.astype(np.float32).reshape(n, 1), n, 1)
+    ih = None if h is None else eng.upload(h.astype(np.float32).reshape(n, 1), n, 1)
+    out, _ = eng.token_logprobs_backward(ix, ii, ls, None if h is None else en, ig, ih, scale, o_bf16)
+    got = orc.from_bf16(eng.download_bf16(out)) if o_bf16 else eng.download(out)
+    lse, ent = eng.download(ls)[:, 0], eng.download(en)[:, 0]
+    for i in [ix, ii, lp, en, ls, ig, out] + ([] if ih is None else [ih]):
+        eng.free(i)
+    return x, got.astype(np.float64), lse, ent
+
+
+@pytest.mark.parametrize("bf16,o_bf16", [(False, False), (True, True), (True, False), (False, True)])
+@pytest.mark.parametrize("cols", [5, 33, 1003, 20011])
+def test_padding_rows_have_no_gradient_whatever_they_hold(eng, cols, bf16, o_bf16):
+    rng = np.random.default_rng(cols)
+    x = logits(rng, 8, cols)
+    x[1] = np.nan
+    x[3, cols // 2] = np.nan
+    x[4, 0] = np.inf
+    x[5] = -np.inf
+    x[6] = np.inf
+    ids = np.array([0, -1, cols - 1, -1, -1, -1, -1, -1])
+    g = rng.standard_normal(8)
+    for h in (None, np.zeros(8)):
+        x_, got, lse, ent = gradient(eng, x, ids, g, h, 1.0, bf16, o_bf16)
+        assert not got[[1, 3, 4, 5, 6, 7]].any()
+        want, tol = grad64(x_[[0, 2]], ids[[0, 2]], lse[[0, 2]], ent[[0, 2]], g.astype(np.float32)[[0, 2]], None, 1.0)
+        assert np.all(np.abs(got[[0, 2]] - want) <= tol + (2.0 ** -8 if o_bf16 else 2 * U) * np.abs(want) + 2.0 ** -126)
