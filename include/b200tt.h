@@ -504,7 +504,8 @@ int32_t b200_token_logprobs(b200_engine*, b200_buffer logits, b200_buffer ids, f
 /* The gradient of the first two with respect to the logits: with p = exp(y - lse) and the rows' upstream gradients
  * d_logprob and d_entropy (F32, rows values; d_entropy and entropy 0: absent),
  *   out = scale * (d_logprob (1[column = id] - p) - d_entropy p (y - lse + entropy)),
- * F32 or rounded once to BF16, [rows, vocab].  lse and entropy are the forward's.  A row whose id is -1 has no d_logprob
+ * F32 or rounded once to BF16, [rows, vocab].  lse and entropy are the forward's; p carries the rounding of lse, |lse| 2^-24 of it,
+ * and from |lse| = 4096 on (a row masked by the type's lowest values, say) log p is taken from the row itself.  A row whose id is -1 has no d_logprob
  * term, and is zero whatever its logits hold where d_entropy is absent or 0 too; an entry of -inf has gradient 0 (its own
  * 1[column = id] term apart), a row of -inf only is zero.  Refused as the forward is. */
 int32_t b200_token_logprobs_backward(b200_engine*, b200_buffer logits, b200_buffer ids, b200_buffer lse, b200_buffer entropy,

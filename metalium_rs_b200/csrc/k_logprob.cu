@@ -13,12 +13,12 @@
 
 #include "device_math.cuh"
 #include "kernels.h"
+#include "pages.cuh"
 #include "pdl.cuh"
 
 namespace b200 {
 namespace {
 
-constexpr int DOMAIN_ERROR = 6;
 constexpr int CLUSTER = 8;               // blocks that share a row, at most
 constexpr int TOP = 32;                  // alternatives a row, at most
 constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
@@ -567,6 +567,39 @@ __device__ __forceinline__ void load_group(const LogprobGradArgs& g, uint64_t at
 #pragma unroll
   for (int i = 0; i < 4; ++i) v[i] = pair_of(x[2 * i], x[2 * i + 1]);
 }
+// Part `segment` of a row whose lse is too large to hold the logarithm of its sum (at 4096 F32's step is 2^-11, and in a row masked
+// by the type's lowest values nothing of it is left): log p is taken again, from differences to the row's largest as the forward
+// takes it.  Rare, so every block of the row reads all of it, and it is out of the way.
+constexpr float FAR = 4096.f;
+template <bool BF, bool OUT_BF>
+__device__ __noinline__ void far_row(const LogprobGradArgs& g, uint64_t base, uint32_t segment, uint32_t segments, float h, float H, float up, uint32_t hot) {
+  __shared__ float parts[8];
+  const uint32_t cols = (uint32_t)g.cols, tid = threadIdx.x, warps = blockDim.x / 32;
+  float high = -INFINITY, s = 0.f;
+  for (uint32_t j = tid; j < cols; j += blockDim.x) high = fmaxf(high, load_float(g.logits, base + j, BF));
+#pragma unroll
+  for (int o = 16; o; o >>= 1) high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, o));
+  if (tid % 32 == 0) parts[tid / 32] = high;
+  __syncthreads();
+  for (uint32_t w = 0; w < warps; ++w) high = fmaxf(high, parts[w]);
+  __syncthreads();
+  for (uint32_t j = tid; j < cols; j += blockDim.x) s += expf((load_float(g.logits, base + j, BF) - high) * g.scale);
+#pragma unroll
+  for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  if (tid % 32 == 0) parts[tid / 32] = s;
+  __syncthreads();
+  s = 0.f;
+  for (uint32_t w = 0; w < warps; ++w) s += parts[w];
+  const float log_sum = logf(s);
+  const uint32_t each = (cols + segments - 1) / segments, first = segment * each, end = first + each < cols ? first + each : cols;
+  for (uint32_t j = first + tid; j < end; j += blockDim.x) {
+    const float z = (load_float(g.logits, base + j, BF) - high) * g.scale - log_sum, p = expf(z);
+    float v = p == 0.f ? 0.f : p * fmaf(h, z + H, -up);
+    v = high == -INFINITY ? 0.f : (j == hot ? v + up : v);                    // -inf only
+    store_float(g.out, base + j, OUT_BF, v);
+  }
+}
+
 template <bool BF, bool OUT_BF, bool ENTROPY>
 __global__ void __launch_bounds__(256) token_logprobs_backward_kernel(const __grid_constant__ LogprobGradArgs g, uint32_t segments, int vec) {
   pdl_enter();
@@ -585,8 +618,11 @@ __global__ void __launch_bounds__(256) token_logprobs_backward_kernel(const __gr
   if (!named && id != -1 && threadIdx.x == 0) atomicCAS(g.err, 0, DOMAIN_ERROR);
   const float up = named ? given : 0.f;
   const uint32_t hot = named ? (uint32_t)id : 0xffffffffu;
-  // a row of -inf only, and a row with neither gradient (a padding row, whatever its logits hold: 0 * NaN is NaN)
-  const bool empty = lse == -INFINITY || (!named && (!ENTROPY || h == 0.f));
+  const bool empty = !named && (!ENTROPY || h == 0.f);       // a padding row, whatever its logits hold (0 * NaN is NaN)
+  if (!empty && fabsf(lse) >= FAR) {
+    far_row<BF, OUT_BF>(g, base, segment, segments, h, H, up, hot);
+    return;
+  }
   const float flat = ENTROPY ? fmaf(h, H, -up) : -up;
   // p (h (z + H) - up), z = y - lse; with a z below -1000, where p is 0, its factor stays finite
   const auto value = [&](uint64_t v, float& v0, float& v1) {

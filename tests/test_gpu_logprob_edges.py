@@ -134,3 +134,40 @@ def test_padding_rows_have_no_gradient_whatever_they_hold(eng, cols, bf16, o_bf1
         assert not got[[1, 3, 4, 5, 6, 7]].any()
         want, tol = grad64(x_[[0, 2]], ids[[0, 2]], lse[[0, 2]], ent[[0, 2]], g.astype(np.float32)[[0, 2]], None, 1.0)
         assert np.all(np.abs(got[[0, 2]] - want) <= tol + (2.0 ** -8 if o_bf16 else 2 * U) * np.abs(want) + 2.0 ** -126)
+
+
+@pytest.mark.parametrize("bf16,o_bf16", [(False, False), (True, True), (False, True)])
+@pytest.mark.parametrize("rows,cols", [(9, 7), (9, 1003), (9, 20011), (400, 257)])
+def test_gradient_of_rows_whose_lse_holds_no_log(eng, rows, cols, bf16, o_bf16):
+    # From 4096 on F32's step is 2^-11 and more, at 2^20 an eighth: the sum's logarithm, and with it p, is not in lse.  The gradient
+    # is that of the definition: p within 600 u, an entropy's factor within 600 u (1 + entropy + its own |log p|).
+    rng = np.random.default_rng(rows + cols)
+    low = orc.from_bf16(np.array([0xFF7F], np.uint16))[0] if bf16 else np.finfo(np.float32).min
+    x = logits(rng, rows, cols)
+    x[0], x[1], x[2] = low, -1.0e30, 1.0e30                  # all alike
+    x[3] = np.where(np.arange(cols) % 3 == 0, -2.0e6, low)
+    x[4] = rng.integers(0, 3, cols) * 2.0 ** 17 + 2.0 ** 21 if bf16 else rng.integers(0, 9, cols) * 0.5 + 3.0e6
+    x[5] = -np.inf
+    x[5, 2] = -3.0e7
+    x[6] = 1.1e6
+    x[7] += 8000
+    ids = rng.integers(0, cols, rows)
+    ids[6] = -1
+    g = rng.standard_normal(rows).astype(np.float32)
+    for h in (None, rng.standard_normal(rows).astype(np.float32)):
+        x_, got, _, _ = gradient(eng, x, ids, g, h, 1.0, bf16, o_bf16)
+        y = x_[:8].astype(np.float64)
+        z = y - y.max(1, keepdims=True)
+        log = z - np.log(np.exp(z).sum(1, keepdims=True))
+        p = np.exp(log)
+        one = np.arange(cols)[None, :] == ids[:8, None]
+        up_ = np.where(ids[:8] >= 0, g[:8], 0.0)[:, None].astype(np.float64)
+        want, tol = up_ * (one - p), 600 * U * np.abs(up_) * p
+        if h is not None:
+            ent = -np.where(p > 0, p * log, 0).sum(1, keepdims=True)
+            inner = np.where(p > 0, p * (log + ent), 0)
+            want = want - h[:8, None] * inner
+            tol = tol + 600 * U * np.abs(h[:8, None]) * p * (1 + ent + np.where(p > 0, -log, 0)) * 2
+        tol = tol + (2.0 ** -8 if o_bf16 else 4 * U) * (np.abs(want) + tol) + 4 * U * np.abs(up_) * one + 2.0 ** -126
+        off = np.abs(got[:8] - want)
+        assert np.all(off <= tol), (np.argwhere(off > tol)[:4], got[:8][off > tol][:4], want[off > tol][:4])
