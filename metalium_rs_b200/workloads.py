@@ -271,8 +271,7 @@ class LlamaPrefill:
             if len(lengths) != self.batch or len(slots) != self.batch or len(set(slots)) != self.batch or not all(
                     1 <= x <= self.seq for x in lengths) or not all(0 <= s < cache.batch for s in slots):
                 raise ValueError("a paged prefill takes a length of 1 .. seq and a sequence of its own for each prompt")
-            for s, x in zip(slots, lengths):
-                cache.reserve(s, x)
+            cache.reserve_all(slots, lengths)
             place = np.where(np.arange(self.seq)[None, :] < np.array(lengths)[:, None], np.arange(self.seq)[None, :], -1)
             place = e.upload_bits(place.astype(np.int32).reshape(1, -1).view(np.uint32), 1, n, I32)
             owner = e.upload_bits(np.repeat(np.array(slots, np.int32), self.seq).reshape(1, -1).view(np.uint32), 1, n, I32)
@@ -784,15 +783,24 @@ class LlamaPagedDecode:
 
     def reserve(self, slot: int, length: int):
         """Pages for positions 0 .. length - 1 of a slot; MemoryError (and nothing taken) when the pool has not that many."""
-        if length > self.max_len:
-            raise ValueError(f"{length} positions and a cache of {self.max_len}")
-        need = -(-length // self.page_size)
-        have = int((self.tables[slot] >= 0).sum())
-        if need - have > len(self.spare):
-            raise MemoryError(f"{need - have} pages wanted, {len(self.spare)} spare")
-        if need > have:
-            for k in range(have, need):
-                self.tables[slot, k] = self.spare.pop()
+        self.reserve_all([slot], [length])
+
+    def reserve_all(self, slots, lengths):
+        """`reserve` for several slots at once: pages for all of them, or MemoryError and none taken."""
+        if len(set(slots)) != len(slots) or not all(0 <= s < self.batch for s in slots):
+            raise ValueError(f"slots {list(slots)} of {self.batch}, each once")
+        more = []
+        for slot, length in zip(slots, lengths):
+            if length > self.max_len:
+                raise ValueError(f"slot {slot}: {length} positions and a cache of {self.max_len}")
+            more.append(max(0, -(-length // self.page_size) - int((self.tables[slot] >= 0).sum())))
+        if sum(more) > len(self.spare):
+            raise MemoryError(f"{sum(more)} pages wanted for slots {[s for s, k in zip(slots, more) if k]}, {len(self.spare)} spare")
+        for slot, k in zip(slots, more):
+            have = int((self.tables[slot] >= 0).sum())
+            for at in range(have, have + k):
+                self.tables[slot, at] = self.spare.pop()
+        if any(more):
             self._push()
 
     def _push(self):

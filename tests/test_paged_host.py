@@ -1,0 +1,34 @@
+"""`LlamaPagedDecode`'s bookkeeping without a GPU: the pool's pages, slots that come and go, what a failed call leaves behind.  The
+engine is the host-only one, every launch a no-op."""
+import numpy as np
+import pytest
+
+from metalium_rs_b200 import I32, workloads as W
+from tests.test_serving_host import e, fake  # noqa: F401 (fixtures)
+
+CFG = W.LlamaConfig(layers=2, hidden=64, heads=2, kv_heads=1, head_dim=64, ff=128, vocab=256)
+
+
+def decode(e, batch, max_len, pages, page_size, seq=32, prompts=2):  # noqa: F811
+    pre = W.LlamaPrefill(e, CFG, W.llama_weights(CFG, seed=3), prompts, seq)
+    ids = e.upload_bits(np.zeros((1, prompts * seq), np.int32), 1, prompts * seq, I32)
+    return pre, ids, W.LlamaPagedDecode(e, CFG, pre.w, batch, max_len=max_len, pages=pages, page_size=page_size)
+
+
+def test_a_prefill_the_pool_has_no_room_for_takes_nothing(e):  # noqa: F811
+    pre, ids, paged = decode(e, 3, 64, pages=3, page_size=16)
+    held = e.device_traffic().pool_in_use
+    with pytest.raises(MemoryError, match=r"4 pages.*\[2, 0\].*3 spare"):
+        pre.forward(ids, cache=paged, slots=[2, 0])
+    assert sorted(paged.spare) == [0, 1, 2] and (paged.tables == -1).all() and e.device_traffic().pool_in_use == held
+    with pytest.raises(ValueError, match="slot 1"):
+        paged.reserve_all([0, 1], [16, 65])
+    for slots in ([0, 0], [3], [-1]):
+        with pytest.raises(ValueError, match="each once"):
+            paged.reserve_all(slots, [1] * len(slots))
+    assert len(paged.spare) == 3
+    pre.forward(ids, cache=paged, slots=[2, 0], lengths=[32, 16])
+    assert not paged.spare and (paged.tables >= 0).sum(1).tolist() == [1, 0, 2]
+    paged.finish(2)
+    paged.finish(0)
+    assert sorted(paged.spare) == [0, 1, 2]
