@@ -256,7 +256,7 @@ class LlamaPrefill:
         -- through the fused attention kernel reading keys and values where the cache holds them (whole 128-row
         tiles: start and seq multiples of 128).
         With a `LlamaPagedDecode` as the cache the prompts may be of several lengths (`lengths`, each 1 .. seq; the ids behind
-        a prompt's end are padding) and go to any of its sequences (`slots`, by default 0, 1, ..): rotation and cache write are
+        a prompt's end are padding) and go to any of its idle sequences (`slots`, by default 0, 1, ..): rotation and cache write are
         one op a layer (`rope_append_pages`), padding rows leave the cache as it is, and the logits are those of each prompt's
         last token.  `cache.begin(slots, argmax, lengths)` then goes on from the prompts."""
         e, c, K = self.eng, self.cfg, kinds
@@ -271,6 +271,9 @@ class LlamaPrefill:
             if len(lengths) != self.batch or len(slots) != self.batch or len(set(slots)) != self.batch or not all(
                     1 <= x <= self.seq for x in lengths) or not all(0 <= s < cache.batch for s in slots):
                 raise ValueError("a paged prefill takes a length of 1 .. seq and a sequence of its own for each prompt")
+            live = [s for s in slots if cache.lengths[s] >= 0]
+            if live:
+                raise ValueError(f"slots {live} hold running sequences, which a prompt would overwrite: finish them first")
             cache.reserve_all(slots, lengths)
             place = np.where(np.arange(self.seq)[None, :] < np.array(lengths)[:, None], np.arange(self.seq)[None, :], -1)
             place = e.upload_bits(place.astype(np.int32).reshape(1, -1).view(np.uint32), 1, n, I32)

@@ -32,3 +32,15 @@ def test_a_prefill_the_pool_has_no_room_for_takes_nothing(e):  # noqa: F811
     paged.finish(2)
     paged.finish(0)
     assert sorted(paged.spare) == [0, 1, 2]
+
+
+def test_a_prefill_into_a_running_sequence_is_refused(e):  # noqa: F811
+    pre, ids, paged = decode(e, 3, 64, pages=12, page_size=16)
+    lg, am = pre.forward(ids, cache=paged, slots=[1, 0], lengths=[20, 30])
+    paged.begin([1, 0], am, [20, 30])
+    before = paged.tables.copy()
+    with pytest.raises(ValueError, match=r"\[1\]"):
+        pre.forward(ids, cache=paged, slots=[2, 1])
+    assert np.array_equal(paged.tables, before) and paged.lengths.tolist() == [30, 20, -1]
+    paged.finish(1)
+    pre.forward(ids, cache=paged, slots=[2, 1])
