@@ -778,6 +778,7 @@ class LlamaPagedDecode:
         self.vc = [z() for _ in range(cfg.layers)]
         self.spare = list(range(pages - 1, -1, -1))                      # pages no sequence holds
         self.tables = np.full((batch, -(-max_len // page_size)), -1, np.int32)
+        self.held = np.zeros(batch, np.int64)                            # a slot's pages
         self.lengths = np.full(batch, -1, np.int64)                      # a slot's position, -1: idle
         i32 = lambda a, r, k: eng.upload_bits(np.ascontiguousarray(a, dtype=np.int32).view(np.uint32), r, k, I32)
         self.table = i32(self.tables, *self.tables.shape)
@@ -796,13 +797,13 @@ class LlamaPagedDecode:
         for slot, length in zip(slots, lengths):
             if length > self.max_len:
                 raise ValueError(f"slot {slot}: {length} positions and a cache of {self.max_len}")
-            more.append(max(0, -(-length // self.page_size) - int((self.tables[slot] >= 0).sum())))
+            more.append(max(0, -(-length // self.page_size) - int(self.held[slot])))
         if sum(more) > len(self.spare):
             raise MemoryError(f"{sum(more)} pages wanted for slots {[s for s, k in zip(slots, more) if k]}, {len(self.spare)} spare")
         for slot, k in zip(slots, more):
-            have = int((self.tables[slot] >= 0).sum())
-            for at in range(have, have + k):
-                self.tables[slot, at] = self.spare.pop()
+            for _ in range(k):
+                self.tables[slot, self.held[slot]] = self.spare.pop()
+                self.held[slot] += 1
         if any(more):
             self._push()
 
@@ -829,22 +830,28 @@ class LlamaPagedDecode:
 
     def finish(self, slot: int):
         """The slot becomes idle and its pages go back to the pool."""
-        held = self.tables[slot][self.tables[slot] >= 0]
-        self.spare.extend(int(p) for p in held[::-1])
+        self.spare.extend(self.tables[slot, :self.held[slot]][::-1].tolist())
         self.tables[slot] = -1
+        self.held[slot] = 0
         self.lengths[slot] = -1
         self._push()
         self._set(self.pos, [slot], [-1])
 
     def _reserve_step(self):
-        for s in np.nonzero(self.lengths >= 0)[0]:
-            self.reserve(int(s), int(self.lengths[s]) + 1)
+        # a page for each live slot whose next position starts one: all of them, or an error that names the slots
+        full = np.nonzero(self.lengths >= self.max_len)[0]
+        if full.size:
+            raise ValueError(f"slots {full.tolist()} hold {self.max_len} positions, all that the cache has for one: finish them")
+        short = np.nonzero(self.lengths >= self.held * self.page_size)[0]
+        if short.size:
+            self.reserve_all(short.tolist(), (self.lengths[short] + 1).tolist())
 
     def _advance(self):
         self.lengths[self.lengths >= 0] += 1
 
     def step(self):
-        """One token for every live slot.  Returns {"logits" [batch, vocab], "argmax" [batch, 1] I32, "logprob", "entropy"
+        """One token for every live slot (an error, and nothing changed, where the pool has no page for one of them or a slot is at
+        the cache's last position: it names the slots, and `finish` of one lets the others go on).  Returns {"logits" [batch, vocab], "argmax" [batch, 1] I32, "logprob", "entropy"
         [batch, 1] and, with `top`, "top_ids", "top_logprobs" [batch, top]} buffers, which the caller frees; the rows of idle
         slots mean nothing.  Advances the live slots' positions and feeds the argmax back."""
         self._reserve_step()

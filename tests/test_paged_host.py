@@ -44,3 +44,31 @@ def test_a_prefill_into_a_running_sequence_is_refused(e):  # noqa: F811
     assert np.array_equal(paged.tables, before) and paged.lengths.tolist() == [30, 20, -1]
     paged.finish(1)
     pre.forward(ids, cache=paged, slots=[2, 1])
+
+
+def test_a_step_takes_its_pages_at_once_or_names_the_slots(e):  # noqa: F811
+    pre, ids, paged = decode(e, 4, 10, pages=5, page_size=4)
+    paged.begin([0, 1, 3], [5, 6, 7], [0, 0, 0])
+    writes = lambda: e.device_traffic().h2d_calls  # noqa: E731
+    before = writes()
+    for _ in range(4):
+        paged.step()
+    assert writes() - before == 1 and paged.held.tolist() == [1, 1, 0, 1]       # three first pages, one table
+    with pytest.raises(MemoryError, match=r"3 pages.*\[0, 1, 3\].*2 spare"):
+        paged.step()
+    assert len(paged.spare) == 2 and paged.lengths.tolist() == [4, 4, -1, 4] and paged.held.tolist() == [1, 1, 0, 1]
+    paged.finish(1)
+    before = writes()
+    for _ in range(4):
+        paged.step()
+    assert writes() - before == 1 and paged.lengths.tolist() == [8, -1, -1, 8] and len(paged.spare) == 1
+    with pytest.raises(MemoryError, match=r"2 pages.*\[0, 3\].*1 spare"):
+        paged.step()
+    paged.finish(0)
+    for _ in range(2):
+        paged.step()
+    with pytest.raises(ValueError, match=r"\[3\] hold 10 positions"):               # in the middle of its third page
+        paged.step()
+    assert paged.lengths.tolist() == [-1, -1, -1, 10] and paged.held.tolist() == [0, 0, 0, 3]
+    paged.finish(3)
+    assert sorted(paged.spare) == [0, 1, 2, 3, 4] and (paged.tables == -1).all()
