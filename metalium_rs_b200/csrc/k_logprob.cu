@@ -695,17 +695,21 @@ cudaError_t launch_form(const LogprobArgs& g, int size, cudaStream_t stream) {
 
 template <typename T>
 cudaError_t launch_type(const LogprobArgs& g, cudaStream_t stream) {
-  // A row's blocks: as many as leave every block a slice of some thousand values while the rows alone do not fill the GPU (one F32
-  // row of 49,152 with five alternatives: 8.7 us by a cluster of eight, 16.1 by one block; of 260,000 with twenty: 16 and 65).
+  // A row's blocks: as many as leave every block a slice of some thousand values while there are fewer than two an SM (one F32 row
+  // of 49,152 with five alternatives: 8.7 us by a cluster of eight, 16.1 by one block; of 260,000 with twenty: 16 and 65; 295 BF16
+  // rows of 50,257: 13.1 by two blocks a row, 19.5 by four).
   int size = 1;
-  while (size < CLUSTER && g.rows * size < 296 && g.cols / (size * 2) >= 2048) size *= 2;
+  while (size < CLUSTER && g.rows * size < 148 * 2 && g.cols / (size * 2) >= 2048) size *= 2;
   if (size > 1) return launch_form<T, 256, true>(g, size, stream);
   // A row's threads: what a row's end costs grows with its block, what a thread has in flight is the same, so blocks are small as
   // long as there are enough of them to fill the GPU.  64 MB of BF16 logits with twenty alternatives by 32 / 64 / 128 / 256
   // threads a row, us: rows of 2,000 67 / 64 / 83 / 137, of 4,000 46 / 41 / 50 / 84, of 8,000 35 / 31 / 33 / 50, of 16,000
-  // 49 / 30 / 26 / 33, of 32,000 70 / 35 / 22 / 28; 4,000 rows of 1,000 9 / - / - / 28.
+  // 49 / 30 / 26 / 33, of 32,000 70 / 35 / 22 / 28; 4,000 rows of 1,000 9 / - / - / 28.  Long rows few enough for blocks of 256
+  // to be resident at once, four an SM, take those, by 128 / 256: 400 F32 rows of 49,152 25.9 / 19.4, 592 28.1 / 22.8, 650
+  // 28.6 / 32.4; 400 BF16 rows of 11,000 with twenty alternatives 12.0 / 11.7.
   if (g.cols <= 1024) return launch_form<T, 32, false>(g, 1, stream);
-  return g.cols <= 10000 ? launch_form<T, 64, false>(g, 1, stream) : launch_form<T, 128, false>(g, 1, stream);
+  if (g.cols <= 10000) return launch_form<T, 64, false>(g, 1, stream);
+  return g.rows <= 148 * 4 ? launch_form<T, 256, false>(g, 1, stream) : launch_form<T, 128, false>(g, 1, stream);
 }
 
 }  // namespace
