@@ -120,11 +120,6 @@ __device__ __forceinline__ void mma_tf32(float* c, uint32_t a0, uint32_t a1, uin
 // would lose two bits, all toward zero: 7.6e-7 of a result in place of 5e-7.)
 __device__ __forceinline__ uint32_t tf32_of(float x) { return (__float_as_uint(x) + 0x1000u) & 0xffffe000u; }
 __device__ __forceinline__ uint32_t tf32_rest(float x) { return __float_as_uint(x - __uint_as_float(tf32_of(x))); }
-__device__ __forceinline__ float exp2_fast(float x) {   // the hardware's 2^x: 2 units in the last place, 2^-inf = 0
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
 __device__ __forceinline__ uint32_t bf16x2(float lo, float hi) {
   uint32_t r;
   asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));

@@ -23,11 +23,6 @@ constexpr int CLUSTER = 8;               // blocks that share a row, at most
 constexpr int TOP = 32;                  // alternatives a row, at most
 constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
 
-__device__ __forceinline__ float exp2_fast(float x) {   // the hardware's 2^x: 2 units in the last place, 2^-200 = 0
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
 // A product whose subnormal results are zero: a BF16 result below 2^-126 is stored as zero (`f32_to_bf16_bits`).
 __device__ __forceinline__ float mul_flush(float a, float b) {
   float r;

@@ -1,4 +1,4 @@
-// What the paged cache's kernels share: the check of a page number, element loads and stores.
+// What the serving kernels share: the error word's value, element loads and stores, the exponential, the check of a page number.
 #pragma once
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -18,6 +18,12 @@ __device__ __forceinline__ float load_float(const void* p, uint64_t i, int bf16)
 __device__ __forceinline__ void store_float(void* p, uint64_t i, int bf16, float v) {
   if (bf16) reinterpret_cast<uint16_t*>(p)[i] = f32_to_bf16_bits(__float_as_uint(v));
   else reinterpret_cast<float*>(p)[i] = v;
+}
+
+__device__ __forceinline__ float exp2_fast(float x) {   // the hardware's 2^x: 2 units in the last place, 2^-200 and 2^-inf = 0
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
 }
 
 // The pool row of a position, or -1 (with DOMAIN set) where the page is not one of the pool's.  `p` lies within the table.
