@@ -25,10 +25,11 @@
 // F32: the tensor cores cut what they add to a sum, which over the thousands of tiles of a long sequence is a bias (160
 // sequences of 131,072 positions, values of mean 1: 5.7e-4 of the result summed there, 1.5e-6 summed in F32).
 //
-// Measured, heads of 128 (32 over 8), BF16 cache: 128 sequences of 500 to 8,192 393 us = 5.8 TB/s of keys and values (the
-// copies alone, nothing computed, 378), one of 131,001 105 us = 5.1 TB/s (99), 32 of mixed lengths 66 us = 4.1 TB/s (57): what is left
-// is the way to the first copy (prefix sum, page, row) and the join, about 10 us together.  `mma.sync` and not tcgen05: a head
-// group is eight rows, of which a 128-row tile would waste fifteen sixteenths, and the products are hidden behind the copies.
+// Measured, heads of 128 (32 over 8), BF16 cache: 128 sequences of 500 to 8,192 401 us = 5.7 TB/s of keys and values (the
+// copies alone, nothing computed, 378), one of 131,001 106 us = 5.1 TB/s (99), 32 of 5 to 4,100 67 us = 4.0 TB/s (57): what is left
+// is the way to the first copy (prefix sum, page, row), the last runs and the join, about 15 us together.  `mma.sync` and not
+// tcgen05: its tile could have the positions as its 128 rows and the heads as columns, but what bounds the call is the copies, behind
+// which these products lie, and not the products.
 #include <cfloat>
 #include <cmath>
 #include <cstdint>

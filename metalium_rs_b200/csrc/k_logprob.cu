@@ -261,7 +261,7 @@ __device__ __forceinline__ uint32_t place_of(uint64_t key, const uint64_t* keys,
 // 47.0 and 45.1 (1000 rows are more than one round of blocks then).  Four pieces in the other forms, whose threads have few, and as
 // many blocks as the registers allow (0): more of either costs 16000 rows of 2000 59 -> 70 us and above.
 // What bounds the pass is neither limit alone: half of the issue slots and of the exponents' rate, two thirds of a copy's bytes
-// (2000 x 50257 BF16, 28 warps an SM).
+// (2000 x 50257 BF16, 25 warps an SM on average).
 template <typename T, int THREADS, bool SHARED>
 __global__ void __launch_bounds__(THREADS, THREADS == 128 ? 7 : 0) token_logprobs_kernel(const __grid_constant__ LogprobArgs g) {
   constexpr int WARPS = THREADS / 32, N = Vec<T>::N, HELD = THREADS * 8, AHEAD = THREADS == 128 ? 8 : 4, ASKED = 4;

@@ -133,7 +133,7 @@ __device__ __forceinline__ void store_raw8(void* p, uint64_t i, int to_bf16, con
 // rotation, four columns that stay -- in heads y, y + blockDim.y, ..., so that its cos and sin entries are read once for all of
 // its heads (read again for every head they were twice the projection's bytes).  Four and not eight columns: the entries of eight
 // are 32 registers, and the warps they cost are worth more than the wider loads.  8 prompts of 1000 tokens, 32 and 8 heads of 128
-// in BF16: 39.6 us, 4.6 TB/s (eight columns 47.7; four without the early loads 44.7).
+// in BF16: 39.0 us, 4.6 TB/s (eight columns 47.7; four without the early loads 44.7).
 __global__ void __launch_bounds__(512) rope_append_kernel(const __grid_constant__ AppendArgs g) {
   pdl_enter();
   const uint64_t i = blockIdx.x;
@@ -202,7 +202,9 @@ __global__ void __launch_bounds__(512) rope_append_kernel(const __grid_constant_
   }
 }
 
-// Blocks that start at no 16-byte address, and heads or rotations that are not groups of eight columns: an element a thread.
+// Blocks that start at no 16-byte address, and heads or rotations that are not groups of eight columns: an element a thread.  The 8
+// prompts of 1000 tokens above, their block one column into a wider buffer: 124 us (39.0 by the kernel above): an element
+// costs a division by the head's width and three addresses.
 __global__ void __launch_bounds__(128) rope_append_any_kernel(const __grid_constant__ AppendArgs g) {
   pdl_enter();
   const uint64_t i = blockIdx.x;
