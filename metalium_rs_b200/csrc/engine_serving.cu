@@ -72,6 +72,7 @@ int int_list(b200_engine* e, b200_buffer id, uint64_t n, Buf** b, const char* na
 // The cache both calls read: shape, pages, table.
 int page_view(b200_engine* e, const b200_page_shape* shape, b200_buffer key_pages, b200_buffer value_pages, b200_buffer page_table,
               PageView* v, Spans* spans, const char* what) {
+  if (!shape) return e->fail(B200_UNSUPPORTED, "%s: no shape", what);
   Buf *K = nullptr, *V = nullptr, *T = nullptr;
   int st = e->need(key_pages, &K, what);
   if (!st) st = e->need(value_pages, &V, what);

@@ -72,3 +72,10 @@ def test_a_step_takes_its_pages_at_once_or_names_the_slots(e):  # noqa: F811
     assert paged.lengths.tolist() == [-1, -1, -1, 10] and paged.held.tolist() == [0, 0, 0, 3]
     paged.finish(3)
     assert sorted(paged.spare) == [0, 1, 2, 3, 4] and (paged.tables == -1).all()
+
+
+def test_a_call_without_a_shape_is_refused(e, fake):  # noqa: F811
+    import ctypes as C
+    words = (C.c_uint64 * 19)(*[0] * 19)
+    for call, n in ((0, 19), (1, 17)):
+        assert fake.b200_serving_call(e._e, C.c_int32(call), words, C.c_uint64(n)) == 2
